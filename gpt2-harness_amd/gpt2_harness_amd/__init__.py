@@ -26,10 +26,12 @@ from .quantization import (
     quantize_linear,
     quantize_model,
     quantize_tensor,
+    quantize_tokens,
     save_packed,
     unpack_int4,
 )
 from .sampling import generate
+from .scoring import TokenScores, score_tokens, token_logprobs
 
 __all__ = [
     "BenchRow",
@@ -44,6 +46,7 @@ __all__ = [
     "SCHEMES",
     "SyntheticTokenStream",
     "TARGET_SUFFIXES",
+    "TokenScores",
     "benchmark_generation",
     "generate",
     "generate_graph",
@@ -59,8 +62,11 @@ __all__ = [
     "quantize_linear",
     "quantize_model",
     "quantize_tensor",
+    "quantize_tokens",
     "run_quantization_table",
     "save_packed",
+    "score_tokens",
     "time_call",
+    "token_logprobs",
     "unpack_int4",
 ]

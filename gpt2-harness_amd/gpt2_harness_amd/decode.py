@@ -21,7 +21,7 @@ Two step implementations:
 * :class:`GraphDecoder`: the model's own modules as torch ops with attention
   over all ``T_max`` slots, the slots after the current position masked to
   ``-inf`` (probability exactly 0), for models the fused step does not take
-  (unquantized or partly quantized blocks, other head widths).
+  (unquantized or partly quantized blocks, int8 activations, other head widths).
 
 Greedy token ids are the reference's; logits agree with an eager forward to
 fp32 rounding.
@@ -34,7 +34,7 @@ import math
 import torch
 
 from . import _lib
-from .qlinear import FMT_W4, FMT_W4G, FMT_W8, QuantLinear
+from .qlinear import FMT_W4, FMT_W4G, FMT_W8, FMT_W8A8, QuantLinear
 
 __all__ = ["FusedDecoder", "GraphDecoder", "generate_graph", "make_decoder"]
 
@@ -187,9 +187,13 @@ def fused_supported(model) -> str | None:
         for lin in (block.attn.c_attn, block.attn.c_proj, block.mlp.c_fc, block.mlp.c_proj):
             if not isinstance(lin, QuantLinear):
                 return "every target Linear must be quantized"
+            if lin.fmt == FMT_W8A8:
+                return "the fused step keeps fp32 activations"
     head = model.lm_head
     if model.wte.weight.dtype != torch.float32 or head.bias is not None:
         return "needs an fp32 embedding and a bias-free lm_head"
+    if isinstance(head, QuantLinear) and head.fmt == FMT_W8A8:
+        return "the fused step keeps fp32 activations"
     if not isinstance(head, QuantLinear) and head.weight.dtype != torch.float32:
         return "needs an fp32 or quantized lm_head"
     return None

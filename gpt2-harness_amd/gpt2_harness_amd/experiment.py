@@ -80,7 +80,8 @@ def run_quantization_table(
     batch_size: int = 4,
     speed: bool = True,
     device: str | torch.device = "cuda",
-    schemes: tuple[tuple[str, int, str, bool], ...] = SCHEMES,
+    schemes: tuple[tuple, ...] = SCHEMES,
+    token_scores: bool = False,
 ) -> dict[str, Any]:
     """Score the fp32 ``model`` and each scheme of ``schemes`` on ``dataset``.
 
@@ -88,15 +89,20 @@ def run_quantization_table(
     (the reference's ``TokenDataset`` or
     :class:`~gpt2_harness_amd.quantization.SyntheticTokenStream`). Returns
     ``{"baseline": {...}, "rows": [QuantResult.to_dict(), ...], "meta": {...}}``.
+    A scheme may carry a fifth entry, the bits of its activations (``None`` or 8, as
+    ``quantize_model``'s ``act_bits``). ``token_scores``: every quality also holds
+    the mean entropy and the top-1 accuracy.
     """
     device = torch.device(device)
     model = model.to(device).eval()
-    scoring = dict(n_chunks=n_chunks, batches_per_chunk=batches_per_chunk, batch_size=batch_size, device=device)
+    scoring = dict(n_chunks=n_chunks, batches_per_chunk=batches_per_chunk, batch_size=batch_size, device=device,
+                   token_scores=token_scores)
     base = perplexity_with_error_bars(model, dataset, **scoring)
     baseline = {**base, "bytes": model_size_bytes(model), "speed": _speed(model, device, speed)}
     rows = []
-    for label, bits, granularity, with_embedding in schemes:
-        qm, stats = quantize_model(model, bits, granularity, include_embedding=with_embedding)
+    for label, bits, granularity, with_embedding, *act_bits in schemes:
+        qm, stats = quantize_model(model, bits, granularity, include_embedding=with_embedding,
+                                   act_bits=act_bits[0] if act_bits else None)
         quality = perplexity_with_error_bars(qm, dataset, **scoring)
         quality["paired_loss_delta"] = paired_loss_delta(quality["chunk_losses"], base["chunk_losses"])
         rows.append(QuantResult(label, bits, granularity, with_embedding, stats, quality,

@@ -11,7 +11,9 @@ codes from HBM and dequantize them in registers.
 The call contract of the slot is unchanged: ``module(x)`` with ``x`` of shape
 ``(..., in_features)`` returns ``(..., out_features)``. fp32 activations give an
 fp32 result accumulated in fp32 (the decode path used for greedy parity);
-bf16 activations give a bf16 result (fp32 accumulation), the W8A16 path.
+bf16 activations give a bf16 result (fp32 accumulation), the W8A16 path. The
+``w8a8`` format quantizes the activations too, each token's row when it arrives
+(:func:`~gpt2_harness_amd.quantization.quantize_tokens`), and multiplies integers.
 ``weight`` returns the dequantized ``W_hat`` the reference would hold.
 """
 
@@ -22,7 +24,7 @@ import torch.nn as nn
 
 from . import _lib
 
-FMT_W8, FMT_W4, FMT_W4G = "int8", "int4", "int4_groupwise"
+FMT_W8, FMT_W4, FMT_W4G, FMT_W8A8 = "int8", "int4", "int4_groupwise", "w8a8"
 _WF = {FMT_W8: _lib.WF_INT8, FMT_W4: _lib.WF_INT4, FMT_W4G: _lib.WF_INT4G}
 
 
@@ -31,9 +33,11 @@ class QuantLinear(nn.Module):
 
     Args:
         codes: ``(N, K)`` int8 codes (``fmt='int8'``), the reference nibble
-            layout ``(N * K / 2,)`` uint8 (``fmt='int4'``), or ``(N, ceil(K/2))``
-            uint8 group-wise nibbles (``fmt='int4_groupwise'``).
-        scale: ``(N,)`` fp32 per-row scales (``int8``/``int4``) or
+            layout ``(N * K / 2,)`` uint8 (``fmt='int4'``), ``(N, ceil(K/2))``
+            uint8 group-wise nibbles (``fmt='int4_groupwise'``), or ``(N, K)``
+            int8 codes that the module keeps as operand tiles (``fmt='w8a8'``:
+            activations are quantized to int8 as well).
+        scale: ``(N,)`` fp32 per-row scales (``int8``/``int4``/``w8a8``) or
             ``(N, ceil(K/group))`` fp16 group scales.
         bias: ``(N,)`` fp32 or ``None``.
         in_features / out_features: ``K`` / ``N``.
@@ -61,7 +65,7 @@ class QuantLinear(nn.Module):
         self.granularity = granularity
         self.fmt = fmt
         self.group_size = int(group_size)
-        self.register_buffer("codes", codes.contiguous())
+        self.register_buffer("codes", tile_codes(codes) if fmt == FMT_W8A8 else codes.contiguous())
         self.register_buffer("scale", scale.contiguous())
         if bias is not None:
             self.bias = nn.Parameter(bias.detach().to(torch.float32).contiguous(), requires_grad=False)
@@ -100,7 +104,7 @@ class QuantLinear(nn.Module):
         without the activation's own pass. None where that entry point does
         not apply; the caller then takes the two steps."""
         K, N = self.in_features, self.out_features
-        if (not x.is_cuda or x.dtype != torch.float32 or x.shape[-1] != K or K % 64
+        if (self.fmt == FMT_W8A8 or not x.is_cuda or x.dtype != torch.float32 or x.shape[-1] != K or K % 64
                 or (torch.is_grad_enabled() and x.requires_grad)):
             return None
         lead = x.shape[:-1]
@@ -128,7 +132,7 @@ class QuantLinear(nn.Module):
 
     def writes_kv(self, M: int) -> bool:
         """Whether :meth:`forward_prefill` over ``M`` rows takes ``kv``."""
-        return bool(_lib.lib().tiq_linear_prefill_writes_kv(_WF[self.fmt], M, self.in_features, self.out_features))
+        return self.fmt != FMT_W8A8 and bool(_lib.lib().tiq_linear_prefill_writes_kv(_WF[self.fmt], M, self.in_features, self.out_features))
 
     def forward_prefill(self, x2: torch.Tensor, ln: nn.LayerNorm | None = None, gelu: bool = False,
                         residual: torch.Tensor | None = None,
@@ -142,7 +146,7 @@ class QuantLinear(nn.Module):
         matrix cores as digit planes; the caller then takes the separate steps."""
         M, K = x2.shape
         N, fmt = self.out_features, self.fmt
-        if M <= 4 or K != self.in_features or (residual is not None and residual.shape[-1] != N):
+        if fmt == FMT_W8A8 or M <= 4 or K != self.in_features or (residual is not None and residual.shape[-1] != N):
             return None
         L = _lib.lib()
         ws_bytes = L.tiq_linear_workspace(_WF[fmt], _lib.F32, M, K, N)
@@ -182,6 +186,8 @@ class QuantLinear(nn.Module):
 
 def linear_into(m: QuantLinear, x2: torch.Tensor, y: torch.Tensor) -> None:
     """``y = x2 @ W_hat^T + b`` into a preallocated ``(M, N)`` tensor."""
+    if m.fmt == FMT_W8A8:
+        return _w8a8_into(m, x2, y)
     L = _lib.lib()
     M, K = x2.shape
     N, fmt = m.out_features, m.fmt
@@ -208,12 +214,51 @@ def linear_into(m: QuantLinear, x2: torch.Tensor, y: torch.Tensor) -> None:
         _lib.check(rc, f"quantized linear ({fmt}, M={M}, K={K}, N={N})")
 
 
+def tile_codes(codes: torch.Tensor) -> torch.Tensor:
+    """``(N, K)`` int8 codes as the 32 x 32 operand tiles of the ``w8a8`` product
+    (``tiq_w8a8_tile``; zeros past N and K), a flat int8 tensor."""
+    if codes.dim() != 2 or codes.dtype != torch.int8:
+        raise ValueError(f"w8a8 expects 2-D int8 codes, got {codes.dtype} {tuple(codes.shape)}")
+    codes = codes.contiguous()
+    N, K = codes.shape
+    with torch.cuda.device(codes.device):
+        L = _lib.lib()
+        tiles = torch.empty(L.tiq_w8a8_tiles_bytes(N, K), dtype=torch.int8, device=codes.device)
+        _lib.check(L.tiq_w8a8_tile(codes.data_ptr(), N, K, K, tiles.data_ptr(), _lib.stream_of(codes)), "w8a8 tiles")
+    return tiles
+
+
+def _w8a8_into(m: QuantLinear, x2: torch.Tensor, y: torch.Tensor) -> None:
+    """The ``w8a8`` product: ``x2``'s rows quantized, then multiplied as integers."""
+    codes, scale, bias = m._buffers["codes"], m._buffers["scale"], m._parameters["bias"]
+    dev = x2.get_device()
+    if codes.get_device() != dev:
+        raise RuntimeError(f"input is on {x2.device}, the quantized weight on {codes.device}")
+    if dev != torch._C._cuda_getDevice():  # launches go to the current device
+        with torch.cuda.device(dev):
+            return _w8a8_into(m, x2, y)
+    L = _lib.lib()
+    M, K = x2.shape
+    N = m.out_features
+    ws_bytes = L.tiq_linear_w8a8_workspace(M, K, N)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x2.device)
+    rc = L.tiq_linear_w8a8(x2.data_ptr(), _lib.dtype_code(x2.dtype), M, K, x2.stride(0), codes.data_ptr(),
+                           scale.data_ptr(), None if bias is None else bias.data_ptr(), N, y.data_ptr(),
+                           _lib.dtype_code(y.dtype), y.stride(0), ws.data_ptr(), ws_bytes, _lib.stream_of(x2))
+    if rc:
+        _lib.check(rc, f"quantized linear (w8a8, M={M}, K={K}, N={N})")
+
+
 def dequantize(m: QuantLinear) -> torch.Tensor:
     L = _lib.lib()
     N, K = m.out_features, m.in_features
     out = torch.empty((N, K), dtype=torch.float32, device=m.codes.device)
     st = _lib.stream_of(out)
-    if m.fmt == FMT_W8:
+    if m.fmt == FMT_W8A8:
+        codes = torch.empty((N, K), dtype=torch.int8, device=m.codes.device)
+        _lib.check(L.tiq_w8a8_untile(m.codes.data_ptr(), N, K, codes.data_ptr(), st), "w8a8 codes")
+        rc = L.tiq_dequantize_int8(codes.data_ptr(), m.scale.data_ptr(), 1, N, K, out.data_ptr(), st)
+    elif m.fmt == FMT_W8:
         rc = L.tiq_dequantize_int8(m.codes.data_ptr(), m.scale.data_ptr(), 1, N, K, out.data_ptr(), st)
     elif m.fmt == FMT_W4:
         rc = L.tiq_dequantize_int4(m.codes.data_ptr(), m.scale.data_ptr(), 1, N, K, out.data_ptr(), st)

@@ -22,7 +22,8 @@ Same public names, argument meaning and error messages as the reference's
 
 Everything runs on the GPU: tensors must live on a ROCm device, and the
 functions raise when the HIP library is missing. Group-wise int4 with fp16
-scales (``group_size=``) is an extension with no counterpart in the reference.
+scales (``group_size=``) and int8 activations (``act_bits=``,
+:func:`quantize_tokens`) are extensions with no counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -40,7 +41,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
-from .qlinear import FMT_W4, FMT_W4G, FMT_W8, QuantLinear
+from .qlinear import FMT_W4, FMT_W4G, FMT_W8, FMT_W8A8, QuantLinear
+from .scoring import token_logprobs
 
 __all__ = [
     "TARGET_SUFFIXES",
@@ -54,6 +56,7 @@ __all__ = [
     "quantize_linear",
     "quantize_model",
     "quantize_tensor",
+    "quantize_tokens",
     "load_packed",
     "save_packed",
     "unpack_int4",
@@ -185,16 +188,63 @@ def quantize_groupwise_int4(w: torch.Tensor, group_size: int = 128) -> tuple[tor
     return packed, scale
 
 
+def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """int8 codes of activations, one scale a token (no counterpart in the reference).
+
+    Args:
+        x: ``(..., K)`` fp32 or bf16 activations on the GPU.
+
+    Returns:
+        ``(q, scale)``: int8 codes shaped like ``x`` and fp32 scales ``(..., 1)``,
+        bit-identical to ``quantize_tensor(x.float(), 8)`` on the rows. This is what
+        a ``w8a8`` :class:`QuantLinear` multiplies; the module quantizes its input
+        itself.
+    """
+    _lib.require_gpu(x, "x")
+    code = _lib.dtype_code(x.dtype)
+    if x.dim() == 0:
+        raise ValueError("quantize_tokens expects rows, got a scalar")
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+    K = x.shape[-1]
+    if K == 0:
+        raise RuntimeError("amax(): cannot reduce over an empty row")
+    if q.numel():
+        x2 = x.reshape(-1, K)
+        if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < K):
+            x2 = x2.contiguous()
+        with torch.cuda.device(x.device):
+            rc = _lib.lib().tiq_quantize_tokens(x2.data_ptr(), code, x2.shape[0], K, max(x2.stride(0), K),
+                                                q.data_ptr(), K, scale.data_ptr(), _lib.stream_of(x2))
+        _lib.check(rc, "quantize_tokens")
+    return q, scale
+
+
+def _check_act_bits(act_bits: int | None, group_size: int | None) -> None:
+    if act_bits is None:
+        return
+    if act_bits != 8:
+        raise ValueError(f"activations are quantized to 8 bits only, got act_bits={act_bits}")
+    if group_size is not None:
+        raise ValueError("int8 activations need one scale a channel, not group_size")
+
+
 def quantize_linear(
-    linear: nn.Linear, bits: int, granularity: Granularity = "per_channel", group_size: int | None = None
+    linear: nn.Linear,
+    bits: int,
+    granularity: Granularity = "per_channel",
+    group_size: int | None = None,
+    act_bits: int | None = None,
 ) -> tuple[QuantLinear, tuple[torch.Tensor, torch.Tensor]]:
-    """Build the :class:`QuantLinear` replacing ``linear``.
+    """Build the :class:`QuantLinear` replacing ``linear`` (``act_bits=8``: with its
+    activations quantized per token, ``quantize_tokens``).
 
     Returns ``(module, (q, scale))`` where ``(q, scale)`` are the reference's
     ``quantize_tensor`` outputs (kept for :func:`packed_size_bytes`); for the
     group-wise format they are the packed nibbles and the fp16 scales.
     """
     _check_bits_granularity(bits, granularity)
+    _check_act_bits(act_bits, group_size)
     w = linear.weight.detach().float()
     N, K = w.shape
     bias = None if linear.bias is None else linear.bias.detach()
@@ -205,15 +255,18 @@ def quantize_linear(
         mod = QuantLinear(packed, s16, bias, K, N, bits, f"group{group_size}", FMT_W4G, group_size)
         return mod, (packed, s16)
     q, scale = quantize_tensor(w, bits, granularity)
-    return _quant_linear_from_codes(q, scale, bias, bits, granularity), (q, scale)
+    return _quant_linear_from_codes(q, scale, bias, bits, granularity, act_bits), (q, scale)
 
 
 def _quant_linear_from_codes(q: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None, bits: int,
-                             granularity: str) -> QuantLinear:
+                             granularity: str, act_bits: int | None = None) -> QuantLinear:
     """The storage :func:`quantize_linear` picks for ``(q, scale)`` of an
-    ``(N, K)`` weight: nibbles for <= 4 bits and even K, int8 codes otherwise."""
+    ``(N, K)`` weight: operand tiles with int8 activations, nibbles for <= 4 bits
+    and even K, int8 codes otherwise."""
     N, K = q.shape
     row_scale = scale.reshape(-1).expand(N).contiguous() if granularity == "per_tensor" else scale.reshape(N)
+    if act_bits is not None:
+        return QuantLinear(q, row_scale, bias, K, N, bits, granularity, FMT_W8A8)
     if bits <= 4 and K % 2 == 0:
         return QuantLinear(pack_int4(q), row_scale, bias, K, N, bits, granularity, FMT_W4)
     return QuantLinear(q, row_scale, bias, K, N, bits, granularity, FMT_W8)
@@ -238,6 +291,7 @@ def quantize_model(
     group_size: int | None = None,
     *,
     save_to: str | Path | None = None,
+    act_bits: int | None = None,
 ) -> tuple[nn.Module, dict[str, Any]]:
     """Return a copy of the model with its target Linears quantized.
 
@@ -254,11 +308,16 @@ def quantize_model(
             target Linears (``bits`` must be 4).
         save_to: Extension: also keep the packed checkpoint whose size is
             ``packed_bytes`` at this path (read back by :func:`load_packed`).
+        act_bits: Extension: 8 also quantizes the activations of the target
+            Linears, each token's row when it arrives (``w8a8``; weights of any
+            ``bits`` are then held as int8 codes). The head and the embedding keep
+            float activations.
 
     Returns:
         ``(quantized_model, stats)`` with the reference's stats keys.
     """
     _check_bits_granularity(bits, granularity)
+    _check_act_bits(act_bits, group_size)
     for p in model.parameters():
         _lib.require_gpu(p, "model parameters")
         break
@@ -279,7 +338,7 @@ def quantize_model(
         for name, module in targets:
             w = module.weight.data
             if isinstance(module, nn.Linear):
-                new, code = quantize_linear(module, bits, granularity, group_size)
+                new, code = quantize_linear(module, bits, granularity, group_size, act_bits)
                 _set_submodule(q_model, name, new)
             else:
                 tied = _tied_head(q_model)
@@ -308,6 +367,8 @@ def quantize_model(
     stats["compression_ratio"] = stats["fp32_bytes"] / stats["packed_bytes"]
     if group_size is not None:
         stats["group_size"] = group_size
+    if act_bits is not None:
+        stats["act_bits"] = act_bits
     return q_model, stats
 
 
@@ -323,7 +384,8 @@ def _packed_payload(
     ``name.scale`` (fp32), ``name.shape`` (int32 ``[N, K]``), plus every other
     unique parameter in fp32. The group-wise format (no counterpart in the
     reference) stores its per-row nibbles, fp16 group scales, the true
-    ``[N, K]`` and ``name.group`` (int32).
+    ``[N, K]`` and ``name.group`` (int32); a Linear with int8 activations adds
+    ``name.act_bits`` (int32).
     """
     payload: dict[str, torch.Tensor] = {}
     for name, (q, scale) in codes.items():
@@ -337,6 +399,8 @@ def _packed_payload(
         payload[f"{name}.q"] = (pack_int4(q) if bits == 4 else q).cpu()
         payload[f"{name}.scale"] = scale.to(torch.float32).cpu()
         payload[f"{name}.shape"] = torch.tensor(list(q.shape), dtype=torch.int32)
+        if getattr(model.get_submodule(name), "fmt", None) == FMT_W8A8:
+            payload[f"{name}.act_bits"] = torch.tensor(8, dtype=torch.int32)
 
     quantized_weight_names = {f"{n}.weight" for n in codes}
     seen: set[int] = set()
@@ -432,7 +496,9 @@ def load_packed(model: nn.Module, source: str | Path | dict[str, torch.Tensor]) 
             if tied:  # as quantize_model: the head over the same codes
                 model.lm_head = _quant_linear_from_codes(c8, scale, None, bits, granularity)
             continue
-        _set_submodule(model, name, _quant_linear_from_codes(c8, scale, bias, bits, granularity))
+        act_bits = int(payload[f"{name}.act_bits"]) if f"{name}.act_bits" in payload else None
+        _check_act_bits(act_bits, None)
+        _set_submodule(model, name, _quant_linear_from_codes(c8, scale, bias, bits, granularity, act_bits))
     quantized = set(names)
     for pname, p in model.named_parameters():
         owner = pname.rpartition(".")[0]
@@ -487,6 +553,7 @@ def perplexity_with_error_bars(
     batches_per_chunk: int = 2,
     batch_size: int = 4,
     device: str | torch.device = "cuda",
+    token_scores: bool = False,
 ) -> dict[str, Any]:
     """Held-out perplexity with a spread over disjoint chunks (``quantization.py:262-319``).
 
@@ -495,6 +562,12 @@ def perplexity_with_error_bars(
     :class:`SyntheticTokenStream`. The forward passes (prefill-shaped Linears,
     ``M = batch_size * block_size``) and the summed cross entropy run on the
     GPU; the chunk sums come back to the host once, after the last batch.
+
+    ``token_scores`` (an extension): the losses come from
+    :func:`~gpt2_harness_amd.scoring.token_logprobs`, one pass over the logits, and the
+    result also holds ``entropy_mean`` (nats a token) and ``top1_accuracy``. Targets
+    are then token ids, or ``-100`` for one to leave out of the sums and the counts
+    of the two.
     """
     model = model.to(device).eval()
     batches = dataset.sequential_batches("val", batch_size=batch_size, limit=n_chunks * batches_per_chunk)
@@ -504,13 +577,27 @@ def perplexity_with_error_bars(
     n_chunk = -(-len(batches) // batches_per_chunk)
     sums = torch.zeros(n_chunk, dtype=torch.float64, device=device)
     tokens = [0] * n_chunk
+    extra = torch.zeros(3, dtype=torch.float64, device=device)  # entropy, hits, tokens scored
     for i, (x, y) in enumerate(batches):
         logits = model(x.to(device))["logits"].float()
+        if token_scores:
+            target = y.to(logits.device)
+            s = token_logprobs(logits, target, top=1)
+            seen = target != -100
+            sums[i // batches_per_chunk] -= s.logprob.double().sum()
+            extra += torch.stack([(s.entropy.double() * seen).sum(), (s.top_ids[..., 0] == target).sum().double(),
+                                  seen.sum().double()])
+            tokens[i // batches_per_chunk] += y.numel()
+            continue
         nll = F.cross_entropy(logits.flatten(0, -2), y.to(logits.device).flatten(), reduction="sum")
         sums[i // batches_per_chunk] += nll.double()
         tokens[i // batches_per_chunk] += y.numel()
     losses = [s / n for s, n in zip(sums.tolist(), tokens)]
-    return _chunk_spread(losses)
+    out = _chunk_spread(losses)
+    if token_scores:
+        entropy, hits, seen = extra.tolist()
+        out["entropy_mean"], out["top1_accuracy"] = entropy / max(seen, 1.0), hits / max(seen, 1.0)
+    return out
 
 
 def _chunk_spread(losses: list[float]) -> dict[str, Any]:

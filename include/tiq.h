@@ -600,6 +600,76 @@ int tiq_head_argmax_screened_i8(const float* x, int64_t n_embd, const float* ln_
                                 const float* row_coef, int64_t vocab, float* logits, int64_t* out, int64_t* ids,
                                 int64_t ld_ids, int64_t* pos, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------- int8 activations and int8 weights */
+
+/* Per-token quantization of activations: quantize_tensor(x.float(), 8,
+ * "per_channel") (quantization.py:78-116) with a token's row in the place of a
+ * weight's. x (rows, cols) fp32 or bf16 with leading dimension ldx, at any
+ * alignment of its elements; q (rows, cols) int8 codes with leading dimension ldq,
+ * scale (rows) fp32. A row that holds an infinity or NaN gets the scale and the
+ * codes quantize_tensor gives it (codes 0 where x / scale is NaN), so that its
+ * products are NaN. */
+int tiq_quantize_tokens(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq,
+                        float* scale, void* stream);
+
+/* int8 codes (N, K) in the matrix cores' operand order: tiles of 32 rows x 32
+ * columns, tile (t, u) at ((t U + u) 1024), U = 2 ceil(K / 64), byte 16 l + j of it
+ * q[32 t + l % 32][32 u + 16 (l / 32) + j], zero past N or K. (For N % 32 == 0 and
+ * K % 64 == 0 these are the tiles of tiq_tile_int8.) tiles is 16-byte aligned. */
+size_t tiq_w8a8_tiles_bytes(int64_t N, int64_t K);
+int tiq_w8a8_tile(const int8_t* q, int64_t N, int64_t K, int64_t ldq, int8_t* tiles, void* stream);
+/* ... and back to contiguous rows. */
+int tiq_w8a8_untile(const int8_t* tiles, int64_t N, int64_t K, int8_t* q, void* stream);
+
+/* A Linear on int8 activations and int8 weights, the activations quantized in the
+ * call: y = (sum_k qx qw) sx sw + bias with (qx, sx) of each row of x as
+ * tiq_quantize_tokens gives them, w_tiles (tiq_w8a8_tile) and scale (N) the weight's
+ * codes and channel scales. The integer sums are exact (K <= 131072); an output
+ * takes three roundings in fp32 (the sum, times sx, times sw plus the bias) and one
+ * more where y is bf16. No counterpart in the reference: it takes the place of
+ * F.linear on W_hat (model.py:254,319,352,355) where activations may be coded too.
+ * x (M, K) and y (M, N) fp32 or bf16, at any alignment of their elements. The
+ * workspace is 16-byte aligned. */
+size_t tiq_linear_w8a8_workspace(int64_t M, int64_t K, int64_t N);
+int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const int8_t* w_tiles,
+                    const float* scale, const float* bias, int64_t N, void* y, int y_dtype, int64_t ldy,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* -------------------------------------------------------- token scores */
+
+/* Log probabilities of given tokens under rows of logits, the entropy of each row
+ * and its `top` most probable alternatives (log_softmax and gather inside the
+ * reference's F.cross_entropy, model.py:591-597; entropy and alternatives are an
+ * extension). Row (b, r), b < batch, r < rows, starts at logits + b stride_batch +
+ * r stride_row (elements; the vocabulary's stride is 1) and takes place b rows + r
+ * of every other array; fp32 or bf16 logits at any alignment of their elements.
+ *   logprob   log p of the row's token; 0 where the token is ignore_index, NaN
+ *             for any other token outside [0, vocab);
+ *   entropy   -sum_j p_j log p_j, a probability of 0 adding nothing;
+ *   stats     two floats a row for tiq_token_logprobs_grad (may be NULL);
+ *   top_ids, top_logprobs (batch rows, top)  the alternatives in falling order, of
+ *             equal logits the lower index first, NaN above everything; top <= 64
+ *             and <= vocab, NULL where top is 0.
+ * -inf logits are probabilities of 0. A row that holds NaN or +inf, or nothing above
+ * -inf, has NaN scores. fp32 sums; d of log(1 + d) is summed without the row's
+ * maximum, so a log probability near 0 keeps its digits. vocab <= 2^30. */
+size_t tiq_token_logprobs_workspace(int dtype, int64_t rows, int64_t vocab, int top);
+int tiq_token_logprobs(const void* logits, int dtype, int64_t batch, int64_t rows, int64_t stride_batch,
+                       int64_t stride_row, int64_t vocab, const int64_t* tokens, int64_t ignore_index, int top,
+                       float* logprob, float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradient of the scores with respect to the logits, written whole (batch rows,
+ * vocab), contiguous, in the logits' type:
+ *   [j = t] g + sum_i [j = a_i] g_i - p_j (g + sum_i g_i + h (log p_j + entropy))
+ * with g = g_logprob (0 for an ignored token, NaN for one outside the vocabulary),
+ * h = g_entropy, g_i = g_top of alternative a_i; each of the three may be NULL.
+ * The probabilities are computed again from the logits and the forward's stats. */
+int tiq_token_logprobs_grad(const void* logits, int dtype, int64_t batch, int64_t rows, int64_t stride_batch,
+                            int64_t stride_row, int64_t vocab, const int64_t* tokens, int64_t ignore_index,
+                            const float* stats, const float* entropy, const float* g_logprob, const float* g_entropy,
+                            int top, const int64_t* top_ids, const float* g_top, void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
