@@ -63,19 +63,25 @@ __device__ __forceinline__ void load_vec(const uint16_t* p, float* v) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
+constexpr float kFarRef = -3e38f;  // where a running maximum's ref starts
+constexpr float kFarLogit = 2e38f;  // |m| from here on comes too near it
 
-// Running maximum, sum of e and sum of e z of some of a row's logits. m starts at the
-// lowest finite number, so that -inf logits alone leave s = 0 and no inf - inf arises.
+// Running maximum of some of a row's logits, the sum of 2^t and of 2^t t with t = x log2 e
+// - ref. ref is the maximum times log2 e as a float, so t takes one instruction and one
+// rounding; that ref is not m log2 e itself is made good once, at the end.
 struct Sums {
-    float m = kLowest, s = 0.f, s1 = 0.f;
+    float m = kLowest, ref = kFarRef, s = 0.f, st = 0.f;
 
-    // (differences below -200 are probabilities of 0; the clamp keeps 0 (-inf) out of s1)
+    // (t below -300 are probabilities of 0; the clamps keep 0 (-inf) out of st)
     __device__ __forceinline__ void rebase(float to) {
-        const float dm = fmaxf(m - to, -200.f), r = __builtin_amdgcn_exp2f(dm * kLog2e);
-        s1 = r * fmaf(dm, s, s1);
+        const float next = fmaxf(to * kLog2e, kFarRef);
+        const float dt = fmaxf(ref - next, -300.f), r = __builtin_amdgcn_exp2f(dt);
+        st = r * fmaf(dt, s, st);
         s *= r;
         m = to;
+        ref = next;
     }
     template <int N>
     __device__ __forceinline__ void add(const float (&v)[N]) {
@@ -83,15 +89,15 @@ struct Sums {
 #pragma unroll
         for (int i = 0; i < N; ++i) g = fmaxf(g, v[i]);
         rebase(g);
-        float t[2] = {}, t1[2] = {};
+        float a[2] = {}, b[2] = {};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float z = v[i] - g, e = __builtin_amdgcn_exp2f(z * kLog2e);
-            t[i & 1] += e;
-            t1[i & 1] = fmaf(e, fmaxf(z, -200.f), t1[i & 1]);
+            const float t = fmaf(v[i], kLog2e, -ref), e = __builtin_amdgcn_exp2f(t);
+            a[i & 1] += e;
+            b[i & 1] = fmaf(e, fmaxf(t, -300.f), b[i & 1]);
         }
-        s += t[0] + t[1];
-        s1 += t1[0] + t1[1];
+        s += a[0] + a[1];
+        st += b[0] + b[1];
     }
 };
 
@@ -128,238 +134,363 @@ __device__ __forceinline__ float write_scores(const Scores& o, int64_t row, floa
 
 // The `top` largest of the C <= kCap keys in LDS (C >= top, no two alike), each to
 // its rank: key c goes where as many keys are larger.
-template <typename Put>
+template <int T, typename Put>
 __device__ __forceinline__ void select_keys(uint64_t* keys, int C, int top, Put put) {
-    if (threadIdx.x == 0) keys[C] = 0;  // pairs below (the buffer holds kCap + 2)
+    if (threadIdx.x < 8) keys[C + threadIdx.x] = 0;  // eight at a time below (the buffer holds kCap + 8)
     __syncthreads();
-    for (int c = threadIdx.x; c < C; c += kThreads) {
+    for (int c = threadIdx.x; c < C; c += T) {
         const uint64_t mine = keys[c];
         int rank = 0;
-        for (int i = 0; i < C; i += 2) {
-            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(keys + i);
-            rank += (k.x > mine) + (k.y > mine);
+        for (int i = 0; i < C; i += 8) {
+            ulonglong2 k[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = *reinterpret_cast<const ulonglong2*>(keys + i + 2 * e);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rank += (k[e].x > mine) + (k[e].y > mine);
         }
         if (rank < top) put(rank, mine);
     }
 }
 
-// One pass over a row, or over one of S segments of it (`per` vectors each): the sums
-// go on with a running maximum, a thread's elements in batches of kBatch; every quad of
-// threads has a maximum of its own by then, and the top-th largest of the 64 quads'
-// is a bound that at least `top` logits reach. Only the threads whose own maximum
-// reaches it look at their logits again (a few KB, out of L2), and so does the
-// thread that holds the row's maximum, for d.
+// A key for the selection; past the buffer's end only counted.
+__device__ __forceinline__ void hold(uint64_t* keys, int* count, float xj, int j) {
+    const int c = atomicAdd(count, 1);
+    if (c < kCap) keys[c] = place_key(xj, j);
+}
+
+// The top-th largest of 64 numbers in LDS, in every lane.
+__device__ __forceinline__ float kth_of_64(const float* q, int top) {
+    const int lane = threadIdx.x & 63;
+    const float mine = q[lane];
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < 64; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(q + i);
+        rank += (v.x > mine || (v.x == mine && i < lane)) + (v.y > mine || (v.y == mine && i + 1 < lane)) +
+                (v.z > mine || (v.z == mine && i + 2 < lane)) + (v.w > mine || (v.w == mine && i + 3 < lane));
+    }
+    const uint64_t kth = __ballot(rank == top - 1);
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), __builtin_ctzll(kth)));
+}
+
+// With every logit above `bound` of places first .. last - 1 held: of those equal to it
+// the lowest places, up to `top` keys in all (`low`: the bound is the lowest number, and
+// of -inf next). Each wavefront takes a part of the places in their order and stops
+// when it has found enough.
+template <int T, typename TX>
+__device__ __forceinline__ void hold_ties(uint64_t* keys, int* count, const TX* xr, int first, int last, float bound,
+                                          bool low, int top) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = T / 64;
+    for (int pass = 0; pass < (low ? 2 : 1); ++pass) {
+        const float value = pass ? -__builtin_inff() : bound;
+        const int need = top - *count;
+        __syncthreads();
+        const int part = (last - first + W - 1) / W, end = min(last, first + (wave + 1) * part);
+        int found = 0;
+        for (int j0 = first + wave * part; j0 < end && found < need; j0 += 512) {
+            float u[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = logit(xr + min(j0 + 64 * e + lane, end - 1));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int j = j0 + 64 * e + lane;
+                const bool hit = found < need && j < end && u[e] == value;
+                const uint64_t hits = __ballot(hit);
+                // (no more than `need` a wavefront: the first of them are the lowest)
+                if (hit && found + __popcll(hits & ((1ull << lane) - 1)) < need) hold(keys, count, u[e], j);
+                found += __popcll(hits);
+            }
+        }
+        __syncthreads();
+        if (*count >= top) break;
+    }
+}
+
+// The `top` largest keys of places first .. last - 1 without a bound: the largest below
+// the last one, `top` times. Returns how many there are.
+template <int T, typename TX>
+__device__ __forceinline__ int slow_keys(uint64_t* keys, const TX* xr, int first, int last, int top) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t* red = keys + kCap / 2;  // (the first `top` places hold the results)
+    uint64_t below = ~0ull;
+    __syncthreads();
+    int C = 0;
+    for (; C < top; ++C) {
+        uint64_t best = 0;
+        for (int j = first + (int)threadIdx.x; j < last; j += T) {
+            const uint64_t c = place_key(logit(xr + j), j);
+            best = c < below ? max_u64(best, c) : best;
+        }
+#pragma unroll
+        for (int off = 32; off; off >>= 1) best = max_u64(best, __shfl_xor(best, off, 64));
+        uint64_t* r = red + 16 * (C & 1);
+        if (lane == 0) r[wave] = best;
+        __syncthreads();
+        below = 0;
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) below = max_u64(below, r[w]);
+        if (!below) break;  // a segment shorter than `top`
+        if (threadIdx.x == 0) keys[C] = below;
+    }
+    __syncthreads();
+    return C;
+}
+
+// Row (b, r) of the logits, counted through (at most 2^31 - 1 of them).
 template <typename TX>
-__global__ __launch_bounds__(kThreads) void scores_kernel(const TX* __restrict__ x, int64_t rows, int64_t sb, int64_t sr,
-                                                          int V, int S, int per, Scores o, Part* __restrict__ parts,
-                                                          uint64_t* __restrict__ part_keys) {
-    constexpr int VEC = kVec<TX>;
-    constexpr int B = 16 / VEC;  // vectors a batch
-    __shared__ __attribute__((aligned(16))) uint64_t keys[kCap + 2];
-    __shared__ float quad[64];
-    __shared__ float wmax[4], wsum[4], wsum1[4], result[2];
-    __shared__ int wowner[4], owners[kThreads], counts[3];
+__device__ __forceinline__ const TX* row_at(const TX* x, int64_t row, int64_t rows, int64_t sb, int64_t sr) {
+    const unsigned b = (unsigned)row / (unsigned)rows, r = (unsigned)row - b * (unsigned)rows;
+    return x + (int64_t)b * sb + (int64_t)r * sr;
+}
+
+// Where a row lies: logits up to a 16-byte boundary, whole vectors, the rest.
+template <typename TX>
+struct Row {
+    const TX* x;
+    int head, nvec, tail, V;
+    __device__ __forceinline__ Row(const TX* x_, int V_) : x(x_), V(V_) {
+        head = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(TX));
+        nvec = (V - head) / kVec<TX>;
+        tail = V - head - nvec * kVec<TX>;
+    }
+    __device__ __forceinline__ const TX* vec(int v) const { return x + head + (int64_t)v * kVec<TX>; }
+    // the logit outside the vectors that thread t takes, or -1
+    __device__ __forceinline__ int extra(int t, bool is_first, bool is_last) const {
+        if (is_first && t < head) return t;
+        return is_last && t >= kVec<TX> && t - kVec<TX> < tail ? V - tail + t - kVec<TX> : -1;
+    }
+};
+
+// A row, or one of S segments of it (`per` vectors each), in one pass: the sums go on
+// with a running maximum, a thread's logits in batches of B vectors. Each of 64 groups of
+// threads has a maximum of its own by then, and the top-th largest of the 64 is a bound
+// that at least `top` logits reach. Only the threads whose own maximum reaches it look
+// at their logits again (a few KB, out of the cache), and so does the thread that holds
+// the row's maximum, for d. ONE: a batch a thread is the whole of it, and the logits
+// are looked at again in the registers.
+template <typename TX, int T, int B, bool ONE>
+__global__ __launch_bounds__(T) void scores_kernel(const TX* __restrict__ x, int64_t rows, int64_t sb, int64_t sr,
+                                                   int V, int S, int per, Scores o, Part* __restrict__ parts,
+                                                   uint64_t* __restrict__ part_keys) {
+    constexpr int VEC = kVec<TX>, W = T / 64;
+    __shared__ __attribute__((aligned(16))) uint64_t keys[kCap + 8];
+    __shared__ __attribute__((aligned(16))) float group[64];
+    __shared__ float wmax[W], wsum[W], wsum1[W], result[2];
+    __shared__ int wowner[W], owners[ONE ? 1 : T], listed[1], count[1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / (unsigned)S;
     const int seg = (int)(blockIdx.x - row * S);
-    const TX* xr = x + (row / rows) * sb + (row % rows) * sr;
-    // the row: `head` logits up to a 16-byte boundary, whole vectors, the rest
-    const int head = min(V, (int)((16 - ((uintptr_t)xr & 15)) & 15) / (int)sizeof(TX));
-    const int nvec = (V - head) / VEC, tail = V - head - nvec * VEC;
-    const TX* xv = xr + head;
-    const int v0 = seg * per, v1 = min(nvec, v0 + per);
-    // the logit outside the vectors that thread t takes, or -1
-    auto extra_of = [&](int t) {
-        if (seg == 0 && t < head) return t;
-        return seg == S - 1 && t >= VEC && t - VEC < tail ? V - tail + t - VEC : -1;
-    };
-    if (tid < 3) counts[tid] = 0;
+    const Row<TX> r(row_at(x, row, rows, sb, sr), V);
+    const int v0 = seg * per, v1 = min(r.nvec, v0 + per);
+    auto extra_of = [&](int t) { return r.extra(t, seg == 0, seg == S - 1); };
+    if (tid == 0) listed[0] = count[0] = 0;
+    // the row's token and its logit, two trips to memory, beside the logits' first
+    int64_t token = 0;
+    float xt = 0.f;
+    if (S == 1 && tid == 0) {
+        token = o.tokens[row];
+        if (token >= 0 && token < V) xt = logit(r.x + token);
+    }
 
     Sums a;
-    {
-        const int j = extra_of(tid);
-        if (j >= 0) {
-            const float v[1] = {logit(xr + j)};
-            a.add(v);
+    int v = v0 + tid;
+    if constexpr (!ONE) {
+        for (; v + T * (B - 1) < v1; v += T * B) {
+            uint4 raw[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) raw[b] = *reinterpret_cast<const uint4*>(r.vec(v + T * b));
+            float t[VEC * B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) load_vec(reinterpret_cast<const TX*>(&raw[b]), t + VEC * b);
+            a.add(t);
         }
     }
-    int v = v0 + tid;
-    for (; v + kThreads * (B - 1) < v1; v += kThreads * B) {
-        float t[16];
+    // the last batch, and the logits outside the vectors
+    const int je = extra_of(tid);
+    float u[VEC * B + 1];
+    {
+        constexpr uint32_t none = sizeof(TX) == 4 ? 0xff800000u : 0xff80ff80u;  // -inf
+        uint4 raw[B];
 #pragma unroll
-        for (int b = 0; b < B; ++b) load_vec(xv + (int64_t)(v + kThreads * b) * VEC, t + VEC * b);
-        a.add(t);
+        for (int b = 0; b < B; ++b) {
+            raw[b] = make_uint4(none, none, none, none);
+            if (v + T * b < v1) raw[b] = *reinterpret_cast<const uint4*>(r.vec(v + T * b));
+        }
+        u[VEC * B] = je >= 0 ? logit(r.x + je) : -__builtin_inff();
+#pragma unroll
+        for (int b = 0; b < B; ++b) load_vec(reinterpret_cast<const TX*>(&raw[b]), u + VEC * b);
     }
-    for (; v < v1; v += kThreads) {
-        float t[VEC];
-        load_vec(xv + (int64_t)v * VEC, t);
-        a.add(t);
+    if constexpr (ONE) {
+        a.add(u);
+    } else {  // (wavefronts past the end leave vectors out)
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if (v + T * b < v1) {
+                float t[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) t[i] = u[VEC * b + i];
+                a.add(t);
+            }
+        }
+        if (je >= 0) {
+            const float t[1] = {u[VEC * B]};
+            a.add(t);
+        }
     }
 
     // ---- the workgroup's sums
-    const float qm = fmaxf(a.m, dpp_move<0xB1>(a.m));
-    const float q4 = fmaxf(qm, dpp_move<0x4E>(qm));
-    if ((tid & 3) == 0) quad[tid >> 2] = q4;
+    const int top = o.top;
+    if (top) {
+        float q = a.m;
+        if constexpr (W >= 2) q = fmaxf(q, dpp_move<0xB1>(q));
+        if constexpr (W >= 4) q = fmaxf(q, dpp_move<0x4E>(q));
+        if constexpr (W >= 8) q = fmaxf(q, dpp_move<0x141>(q));
+        if constexpr (W >= 16) q = fmaxf(q, dpp_move<0x140>(q));
+        if (tid % W == 0) group[tid / W] = q;
+    }
     const float wm = wave_max_dpp(a.m);
     const uint64_t at = __ballot(a.m == wm);
-    if (lane == 0) wmax[wave] = wm, wowner[wave] = wave * 64 + __builtin_ctzll(at);
+    if (lane == 0) wmax[wave] = wm, wowner[wave] = wave * 64 + (at ? __builtin_ctzll(at) : 0);
     __syncthreads();
-    const float m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-    const int owner = wmax[0] == m ? wowner[0] : wmax[1] == m ? wowner[1] : wmax[2] == m ? wowner[2] : wowner[3];
+    float m = wmax[W - 1];
+    int owner = wowner[W - 1];
+#pragma unroll
+    for (int w = W - 2; w >= 0; --w) {
+        owner = wmax[w] >= m ? wowner[w] : owner;
+        m = fmaxf(m, wmax[w]);
+    }
     const float own_max = a.m;
     a.rebase(m);
-    const float ws = wave_sum_dpp(tid == owner ? 0.f : a.s), ws1 = wave_sum_dpp(a.s1);
-    if (lane == 0) wsum[wave] = ws, wsum1[wave] = ws1;
-    // the owner's logits but one maximum (s of a thread that saw NaN is NaN already)
-    float rest = 0.f;
-    if (wave == 0) {
-        int equal = 0;
-        auto take = [&](float xj) {
-            const float e = __builtin_amdgcn_exp2f((xj - m) * kLog2e);
-            rest += xj == m ? xj - m : e;  // (+inf - +inf: NaN)
-            equal += xj == m;
-        };
-        for (int w = v0 + owner + kThreads * lane; w < v1; w += kThreads * 64) {
+    const float shift = fmaf(m, kLog2e, -a.ref), back = __builtin_amdgcn_exp2f(-shift);  // exp(x - m) = 2^t back
+    const bool far = !(fabsf(m) < kFarLogit);  // a maximum that is infinite, or as low as a mask's
+    // sums of e and e z; the owner's take its logits once more, without one maximum,
+    // whose 1 would swallow what a sure row's others add
+    float mine = tid == owner ? 0.f : a.s * back;
+    float s1 = tid == owner ? 0.f : kLn2 * back * fmaf(-shift, a.s, a.st);
+    float own = 0.f;
+    int equal = 0;
+    auto but_equal = [&](float xj) {  // e of a logit, but of those at the maximum, which are counted
+        const float z = xj - m, e = xj == m ? z : __builtin_amdgcn_exp2f(z * kLog2e);  // (+inf - +inf: NaN)
+        equal += xj == m;
+        s1 = fmaf(e, fmaxf(z, -200.f), s1);
+        return e;
+    };
+    if (far) {
+        mine = s1 = 0.f;
+        for (int w = v0 + tid; w < v1; w += T) {
             float t[VEC];
-            load_vec(xv + (int64_t)w * VEC, t);
+            load_vec(r.vec(w), t);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) take(t[i]);
+            for (int i = 0; i < VEC; ++i) mine += but_equal(t[i]);
+        }
+        if (je >= 0) mine += but_equal(u[VEC * B]);
+        own = (float)equal - (tid == 0 ? 1.f : 0.f);  // nothing above -inf: -1
+    } else if constexpr (ONE) {
+        if (wave == owner >> 6) {
+            const float others = s1;
+#pragma unroll
+            for (int i = 0; i < VEC * B + 1; ++i) own += but_equal(u[i]);
+            own = tid == owner ? own + (float)(equal - 1) : 0.f;
+            s1 = tid == owner ? s1 : others;
+        }
+    } else if (wave == 0) {
+        for (int w = v0 + owner + T * lane; w < v1; w += T * 64) {
+            float t[VEC];
+            load_vec(r.vec(w), t);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) own += but_equal(t[i]);
         }
         const int j = extra_of(owner);
-        if (lane == 0 && j >= 0) take(logit(xr + j));
-        rest = wave_sum_dpp(rest) + (wave_sum_dpp((float)equal) - 1.f);  // nothing above -inf: -1
+        if (lane == 0 && j >= 0) own += but_equal(logit(r.x + j));
+        own = wave_sum_dpp(own) + (wave_sum_dpp((float)equal) - 1.f);
+        own = lane == 0 ? own : 0.f;
+    }
+    const float ws = wave_sum_dpp(mine + own), ws1 = wave_sum_dpp(s1);
+    if (lane == 0) wsum[wave] = ws, wsum1[wave] = ws1;
+    // ---- alternatives: the bound, and the threads that reach it
+    const float bound = top ? kth_of_64(group, top) : 0.f;
+    const bool low = bound <= kLowest;  // fewer than `top` groups saw more: every logit counts
+    const int first = seg == 0 ? 0 : min(r.head + v0 * VEC, V - r.tail), last = seg == S - 1 ? V : r.head + v1 * VEC;
+    // ONE: the keys of a thread's own logits that a test takes
+    auto hold_own = [&](auto takes) {
+        uint64_t hits = 0;
+#pragma unroll
+        for (int i = 0; i < VEC * B + 1; ++i) hits |= (uint64_t)takes(u[i]) << i;
+        if (je < 0) hits &= ~(1ull << VEC * B);
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+            if (v + T * b >= v1) hits &= ~(((1ull << VEC) - 1) << VEC * b);
+        while (hits) {
+            const int i = __builtin_ctzll(hits);
+            hits &= hits - 1;
+            const int j = i == VEC * B ? je : r.head + (v + T * (i / VEC)) * VEC + i % VEC;
+            hold(keys, count, logit(r.x + j), j);
+        }
+    };
+    if (top) {
+        if constexpr (ONE) {
+            if (low || own_max >= bound) hold_own([&](float xj) { return low || xj >= bound; });
+        } else {
+            if (low || own_max >= bound) owners[atomicAdd(&listed[0], 1)] = tid;
+        }
     }
     __syncthreads();
-    const float others = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
-    const float s1 = (wsum1[0] + wsum1[1]) + (wsum1[2] + wsum1[3]);
     if (tid == 0) {
-        const float d = others + rest;
+        float d = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) d += wsum[w], s1 += wsum1[w];
         if (S > 1) {
             parts[blockIdx.x] = {m, d, s1, 0.f};
         } else {
-            const int64_t t = o.tokens[row];
-            const float xt = t >= 0 && t < V ? logit(xr + t) : 0.f;
-            result[0] = write_scores(o, row, m, d, s1, xt, t, V);
+            result[0] = write_scores(o, row, m, d, s1, xt, token, V);
         }
         result[1] = d;
     }
-    const int top = o.top;
     if (!top) return;
-
-    // ---- alternatives: the bound, and what reaches it
-    float bound;
-    {
-        const float mine = quad[lane];
-        int rank = 0;
-#pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(quad + i);
-            rank += (q.x > mine || (q.x == mine && i < lane)) + (q.y > mine || (q.y == mine && i + 1 < lane)) +
-                    (q.z > mine || (q.z == mine && i + 2 < lane)) + (q.w > mine || (q.w == mine && i + 3 < lane));
-        }
-        const uint64_t kth = __ballot(rank == top - 1);
-        bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), __builtin_ctzll(kth)));
-    }
-    const bool low = bound <= kLowest;  // fewer than `top` quads saw more: every logit counts
-    if (low || own_max >= bound) owners[atomicAdd(&counts[0], 1)] = tid;
-    __syncthreads();
-    const int nown = counts[0], slots = (max(v1 - v0, 0) + kThreads - 1) / kThreads + 1;
-    const bool odd = !(result[1] == result[1]);  // NaN or +inf in the row
+    const int nown = ONE ? 0 : listed[0], slots = (max(v1 - v0, 0) + T - 1) / T + 1;
     auto each_again = [&](auto f) {  // f(logit, place) over the logits of the threads listed
-        for (int i = tid; i < nown * slots; i += kThreads) {
+        for (int i = tid; i < nown * slots; i += T) {
             const int t = owners[i / slots], k = i % slots;
             if (k == slots - 1) {
                 const int j = extra_of(t);
-                if (j >= 0) f(logit(xr + j), j);
+                if (j >= 0) f(logit(r.x + j), j);
                 continue;
             }
-            const int w = v0 + t + kThreads * k;
+            const int w = v0 + t + T * k;
             if (w >= v1) continue;
-            float u[VEC];
-            load_vec(xv + (int64_t)w * VEC, u);
+            float t8[VEC];
+            load_vec(r.vec(w), t8);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f(u[e], head + w * VEC + e);
+            for (int e = 0; e < VEC; ++e) f(t8[e], r.head + w * VEC + e);
         }
     };
-    auto hold = [&](float xj, int j) {
-        const int c = atomicAdd(&counts[1], 1);
-        if (c < kCap) keys[c] = place_key(xj, j);
-    };
-    const int first = seg == 0 ? 0 : min(head + v0 * VEC, V - tail), last = seg == S - 1 ? V : head + v1 * VEC;  // the segment
-    if (!odd) {
+    if constexpr (!ONE) {
         each_again([&](float xj, int j) {
-            if (low || xj >= bound) hold(xj, j);
+            if (low || xj >= bound) hold(keys, count, xj, j);
         });
-        __syncthreads();
-        if (counts[1] > kCap) {
-            // more ties than the buffer holds: what lies above the bound, then of
-            // the equals the lowest places (and of -inf, where the bound is the
-            // lowest number), a quarter of the segment a wavefront
-            __syncthreads();
-            if (tid == 0) counts[1] = 0;
-            __syncthreads();
-            each_again([&](float xj, int j) {
-                if (xj > bound) hold(xj, j);
-            });
-            __syncthreads();
-            if (counts[1] <= kCap / 2) {
-                for (int pass = 0; pass < (low ? 2 : 1); ++pass) {
-                    const float value = pass ? -__builtin_inff() : bound;
-                    const int need = top - counts[1];
-                    __syncthreads();
-                    const int part = (last - first + 3) / 4, end = min(last, first + (wave + 1) * part);
-                    int found = 0;
-                    for (int j0 = first + wave * part; j0 < end && found < need; j0 += 512) {
-                        float u[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) u[e] = logit(xr + min(j0 + 64 * e + lane, end - 1));
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int j = j0 + 64 * e + lane;
-                            const bool hit = found < need && j < end && u[e] == value;
-                            if (hit) hold(u[e], j);
-                            found += __popcll(__ballot(hit));
-                        }
-                    }
-                    __syncthreads();
-                    if (counts[1] >= top) break;
-                }
-            }
-        }
     }
     __syncthreads();
-    int C = counts[1];
-    if (odd || C > kCap) {
-        // NaN among the logits, or large ones in a few threads' places only: the
-        // largest key below the last, `top` times
+    const bool odd = !(result[1] == result[1]);  // NaN or +inf in the row
+    if (!odd && count[0] > kCap) {  // more ties than the buffer holds
         __syncthreads();
-        uint64_t below = ~0ull;
-        for (int k = 0; k < top; ++k) {
-            uint64_t best = 0;
-            for (int j = first + tid; j < last; j += kThreads) {
-                const uint64_t c = place_key(logit(xr + j), j);
-                best = c < below ? max_u64(best, c) : best;
-            }
-#pragma unroll
-            for (int off = 32; off; off >>= 1) best = max_u64(best, __shfl_xor(best, off, 64));
-            uint64_t* red = keys + kCap / 2;  // (the first `top` places hold the results)
-            if (lane == 0) red[4 * (k & 1) + wave] = best;
-            __syncthreads();
-            red += 4 * (k & 1);
-            below = max_u64(max_u64(red[0], red[1]), max_u64(red[2], red[3]));
-            if (tid == 0) keys[k] = below;
-        }
-        C = top;
+        if (tid == 0) count[0] = 0;
         __syncthreads();
-        while (C > 0 && keys[C - 1] == 0) --C;  // a segment shorter than `top`
+        if constexpr (ONE) hold_own([&](float xj) { return xj > bound; });
+        else each_again([&](float xj, int j) {
+            if (xj > bound) hold(keys, count, xj, j);
+        });
+        __syncthreads();
+        if (count[0] <= kCap / 2) hold_ties<T>(keys, count, r.x, first, last, bound, low, top);
     }
+    int C = count[0];
+    if (odd || C > kCap) C = slow_keys<T>(keys, r.x, first, last, top);
     if (S > 1) {
         uint64_t* out = part_keys + (int64_t)blockIdx.x * top;
-        for (int k = C + tid; k < top; k += kThreads) out[k] = 0;
-        select_keys(keys, C, top, [&](int k, uint64_t key) { out[k] = key; });
+        for (int k = C + tid; k < top; k += T) out[k] = 0;
+        select_keys<T>(keys, C, top, [&](int k, uint64_t key) { out[k] = key; });
     } else {
         const float L = result[0];
-        select_keys(keys, C, top, [&](int k, uint64_t key) {
+        select_keys<T>(keys, C, top, [&](int k, uint64_t key) {
             o.top_ids[row * top + k] = (uint32_t)~(uint32_t)key;
             o.top_logprobs[row * top + k] = of_order(key >> 32) - m - L;
         });
@@ -371,12 +502,12 @@ template <typename TX>
 __global__ __launch_bounds__(kThreads) void join_kernel(const TX* __restrict__ x, int64_t rows, int64_t sb, int64_t sr,
                                                         int V, int S, Scores o, const Part* __restrict__ parts,
                                                         const uint64_t* __restrict__ part_keys) {
-    __shared__ __attribute__((aligned(16))) uint64_t keys[kCap + 2];
+    __shared__ __attribute__((aligned(16))) uint64_t keys[kCap + 8];
     __shared__ float wmax[4], wsum[4], wsum1[4], result[1];
     __shared__ int wowner[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
-    const TX* xr = x + (row / rows) * sb + (row % rows) * sr;
+    const TX* xr = row_at(x, row, rows, sb, sr);
     const int64_t t = o.tokens[row];
     const float xt = t >= 0 && t < V ? logit(xr + t) : 0.f;
     Part p = {kLowest, -1.f, 0.f, 0.f};
@@ -385,16 +516,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const TX* __restrict__ x
     for (int i = tid; i < S * top; i += kThreads) keys[i] = part_keys[row * S * top + i];
     const float wm = wave_max_dpp(p.m);
     const uint64_t at = __ballot(p.m == wm);
-    if (lane == 0) wmax[wave] = wm, wowner[wave] = wave * 64 + __builtin_ctzll(at);
+    if (lane == 0) wmax[wave] = wm, wowner[wave] = wave * 64 + (at ? __builtin_ctzll(at) : 0);
     __syncthreads();
     const float m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
     const int owner = wmax[0] == m ? wowner[0] : wmax[1] == m ? wowner[1] : wmax[2] == m ? wowner[2] : wowner[3];
-    Sums a;
-    a.m = p.m;
-    a.s = 1.f + p.d;
-    a.s1 = p.s1;
-    a.rebase(m);
-    const float ws = wave_sum_dpp(tid == owner ? p.d : a.s), ws1 = wave_sum_dpp(a.s1);
+    // exp(p.m - m); segments that hold no more than the row's maximum keep NaN of theirs
+    const float z = fmaxf(p.m - m, -200.f), e = __builtin_amdgcn_exp2f(z * kLog2e);
+    const float ws = wave_sum_dpp(tid == owner ? p.d : (1.f + p.d) * e);
+    const float ws1 = wave_sum_dpp(e * fmaf(z, 1.f + p.d, p.s1));
     if (lane == 0) wsum[wave] = ws, wsum1[wave] = ws1;
     __syncthreads();
     if (tid == 0)
@@ -403,19 +532,33 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const TX* __restrict__ x
     if (!top) return;
     __syncthreads();
     const float L = result[0];
-    select_keys(keys, S * top, top, [&](int k, uint64_t key) {
+    select_keys<kThreads>(keys, S * top, top, [&](int k, uint64_t key) {
         o.top_ids[row * top + k] = (uint32_t)~(uint32_t)key;
         o.top_logprobs[row * top + k] = of_order(key >> 32) - m - L;
     });
 }
 
-// Segments of a row: enough workgroups for the chip where rows are few, each with a
-// vector a thread at least, and as many keys as the join holds.
-int segments(int dtype, int64_t rows, int64_t vocab, int top) {
-    const int64_t vectors = vocab / (dtype == TIQ_F32 ? 4 : 8);
-    int64_t S = std::min((vectors + kThreads - 1) / kThreads, (1024 + rows - 1) / rows);
-    S = std::min<int64_t>(S, top ? kCap / top : kThreads);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(S, kThreads));
+// How rows of n vectors are taken. Up to 256 vectors, a wavefront a row; up to 1024, a
+// workgroup of 256 with a batch a thread (5000 rows of 1003 bf16: 8.6 us against 15 with
+// 256 threads a row). Longer rows are cut into segments until there are about 1024
+// workgroups, each of a batch a thread at least, and no more segments than make the
+// join's keys many (64 rows of 131071 bf16 with 20 alternatives, in 8 / 16 segments: the
+// segments 10.7 / 11.5 us, the join 3.9 / 7.5). Uncut rows: 512 threads (4096 rows of
+// 50257 fp32, 256 / 512 / 1024 threads: 152 / 143 / 141 us; bf16 112 / 103 / 109).
+struct Plan {
+    int T, B;  // threads, vectors a batch
+    bool one;  // a batch a thread
+    int S, per;
+};
+Plan plan_of(int dtype, int64_t rows, int64_t vocab, int top) {
+    const int64_t n = std::max<int64_t>(1, vocab / (dtype == TIQ_F32 ? 4 : 8));
+    if (n <= 256) return {64, n <= 64 ? 1 : n <= 128 ? 2 : 4, true, 1, (int)n};
+    if (n <= 1024) return {256, 4, true, 1, (int)n};
+    int64_t S = std::min((n + 1023) / 1024, (1024 + rows - 1) / rows);
+    S = std::max<int64_t>(1, std::min<int64_t>(S, top ? std::max(4, 160 / top) : kThreads));
+    const int per = (int)((n + S - 1) / S);
+    if (S == 1) return {512, 4, false, 1, per};
+    return {256, 4, per <= 1024, (int)S, per};
 }
 
 struct Grads {
@@ -437,25 +580,31 @@ __device__ __forceinline__ float exp_of(float z) {
     return t > -150.f ? fmaf(e * r, 0.693147181f, e) : e;
 }
 
-__device__ __forceinline__ void store_vec(float* p, const float* v) {
-    *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(v);
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4 packed(const float (&v)[4]) {
+    return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
 }
-__device__ __forceinline__ void store_vec(uint16_t* p, const float* v) {
-    *reinterpret_cast<uint4*>(p) =
-        make_uint4(pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7]));
+__device__ __forceinline__ u32x4 packed(const float (&v)[8]) {
+    return u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
 }
 
 // A read and a write of the logits: `per` vectors of a row a workgroup, aligned to the
 // gradient's 16-byte boundaries (the logits' too, unless a caller's strides shift
 // them). Every element as one that no token names; then the few that one does, anew.
-template <typename TX>
+// The last rows go first: they are what the scores' pass left in the 256 MB cache before
+// memory; and a gradient that would not stay there (PAST) is stored past it, which
+// spares whatever reads next the wait for its write-back. 4096 rows of 50257 bf16, the
+// scores' pass and this one, again and again: 105 + 141 us; from the last row 98 + 136;
+// past the cache too 69 + 136.
+template <typename TX, bool PAST>
 __global__ __launch_bounds__(kThreads) void grad_kernel(const TX* __restrict__ x, int64_t rows, int64_t sb, int64_t sr,
                                                         int V, int chunks, int per, Grads o, TX* grad) {
     constexpr int VEC = kVec<TX>;
     const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x / (unsigned)chunks;
-    const int chunk = (int)(blockIdx.x - row * chunks);
-    const TX* xr = x + (row / rows) * sb + (row % rows) * sr;
+    const unsigned id = gridDim.x - 1 - blockIdx.x;  // the last rows first
+    const int64_t row = id / (unsigned)chunks;
+    const int chunk = (int)(id - row * chunks);
+    const TX* xr = row_at(x, row, rows, sb, sr);
     TX* gr = grad + row * V;
     const int head = min(V, (int)((16 - ((uintptr_t)gr & 15)) & 15) / (int)sizeof(TX));
     const int nvec = (V - head) / VEC, tail = V - head - nvec * VEC;
@@ -493,7 +642,9 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const TX* __restrict__ x
             if (v + kThreads * i >= v1) break;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) u[i][e] = plain(u[i][e]);
-            store_vec(gr + head + (int64_t)(v + kThreads * i) * VEC, u[i]);
+            u32x4* dst = reinterpret_cast<u32x4*>(gr + head + (int64_t)(v + kThreads * i) * VEC);
+            if constexpr (PAST) __builtin_nontemporal_store(packed(u[i]), dst);
+            else *dst = packed(u[i]);
         }
     }
     if (chunk == 0) {
@@ -538,22 +689,32 @@ int check_rows(const void* logits, int dtype, int64_t batch, int64_t rows, int64
 using namespace tiq;
 
 template <typename TX>
-static int run_scores(const TX* x, int64_t count, int64_t rows, int64_t sb, int64_t sr, int V, int S, const Scores& o,
-                      void* workspace, hipStream_t st) {
-    const int vectors = V / kVec<TX>;
+static int run_scores(const TX* x, int64_t count, int64_t rows, int64_t sb, int64_t sr, int V, const Plan& p,
+                      const Scores& o, void* workspace, hipStream_t st) {
     Part* parts = static_cast<Part*>(workspace);
-    uint64_t* keys = reinterpret_cast<uint64_t*>(parts + (S > 1 ? count * S : 0));
-    hipLaunchKernelGGL(scores_kernel<TX>, dim3((unsigned)(count * S)), dim3(kThreads), 0, st, x, rows, sb, sr, V, S,
-                       (vectors + S - 1) / S, o, parts, keys);
-    if (S > 1)
-        hipLaunchKernelGGL(join_kernel<TX>, dim3((unsigned)count), dim3(kThreads), 0, st, x, rows, sb, sr, V, S, o,
+    uint64_t* keys = reinterpret_cast<uint64_t*>(parts + (p.S > 1 ? count * p.S : 0));
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(count * p.S)), dim3(p.T), 0, st, x, rows, sb, sr, V, p.S, p.per, o,
+                           parts, keys);
+    };
+    switch (p.T * 100 + p.B * 10 + p.one) {
+        case 6411: go(scores_kernel<TX, 64, 1, true>); break;
+        case 6421: go(scores_kernel<TX, 64, 2, true>); break;
+        case 6441: go(scores_kernel<TX, 64, 4, true>); break;
+        case 25641: go(scores_kernel<TX, 256, 4, true>); break;
+        case 25640: go(scores_kernel<TX, 256, 4, false>); break;
+        case 51240: go(scores_kernel<TX, 512, 4, false>); break;
+        default: return TIQ_EUNSUPPORTED;
+    }
+    if (p.S > 1)
+        hipLaunchKernelGGL(join_kernel<TX>, dim3((unsigned)count), dim3(kThreads), 0, st, x, rows, sb, sr, V, p.S, o,
                            parts, keys);
     return launch_status();
 }
 
 extern "C" size_t tiq_token_logprobs_workspace(int dtype, int64_t rows, int64_t vocab, int top) {
     if (rows <= 0 || vocab <= 0 || top < 0 || top > kMaxTop || rows > 0x7fffffffLL) return 0;
-    const int S = segments(dtype, rows, vocab, top);
+    const int S = plan_of(dtype, rows, vocab, top).S;
     return S > 1 ? (size_t)rows * S * (sizeof(Part) + 8 * top) : 0;
 }
 
@@ -567,16 +728,16 @@ extern "C" int tiq_token_logprobs(const void* logits, int dtype, int64_t batch, 
     const int64_t count = batch * rows;
     const size_t need = tiq_token_logprobs_workspace(dtype, count, vocab, top);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return TIQ_EWORKSPACE;
-    const int S = segments(dtype, count, vocab, top);
+    const Plan p = plan_of(dtype, count, vocab, top);
     const Scores o = {tokens, ignore_index, top, logprob, entropy, stats, top_ids, top_logprobs};
     if (dtype == TIQ_F32)
-        return run_scores(static_cast<const float*>(logits), count, rows, stride_batch, stride_row, (int)vocab, S, o,
+        return run_scores(static_cast<const float*>(logits), count, rows, stride_batch, stride_row, (int)vocab, p, o,
                           workspace, as_stream(stream));
-    return run_scores(static_cast<const uint16_t*>(logits), count, rows, stride_batch, stride_row, (int)vocab, S, o,
+    return run_scores(static_cast<const uint16_t*>(logits), count, rows, stride_batch, stride_row, (int)vocab, p, o,
                       workspace, as_stream(stream));
 }
 
-// Vectors a workgroup: 4 a thread, 16 where that leaves enough workgroups.
+// Four vectors a thread.
 template <typename TX>
 static int run_grad(const TX* x, int64_t count, int64_t rows, int64_t sb, int64_t sr, int V, const Grads& o, TX* grad,
                     hipStream_t st) {
@@ -584,8 +745,10 @@ static int run_grad(const TX* x, int64_t count, int64_t rows, int64_t sb, int64_
     int per = 4 * kThreads;
     int64_t chunks = (vectors + per - 1) / per;
     if (chunks * count > 0x7fffffffLL) per = (int)vectors, chunks = 1;
-    hipLaunchKernelGGL(grad_kernel<TX>, dim3((unsigned)(count * chunks)), dim3(kThreads), 0, st, x, rows, sb, sr, V,
-                       (int)chunks, per, o, grad);
+    // logits and gradient together beyond the cache's 256 MB
+    const bool past = count * V * (int64_t)sizeof(TX) > (128 << 20);
+    hipLaunchKernelGGL((past ? grad_kernel<TX, true> : grad_kernel<TX, false>), dim3((unsigned)(count * chunks)),
+                       dim3(kThreads), 0, st, x, rows, sb, sr, V, (int)chunks, per, o, grad);
     return launch_status();
 }
 

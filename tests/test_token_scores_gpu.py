@@ -519,3 +519,11 @@ def test_refusals(dev):
         rc = L.tiq_token_logprobs(y.data_ptr(), _lib.F32, 1, 1, 0, 50257, 50257, t.data_ptr(), -100, 5, out.data_ptr(),
                                   out.data_ptr(), None, ids.data_ptr(), out.data_ptr(), None, 0, _lib.stream_of(y))
         assert rc == _lib.EWORKSPACE and torch.all(out == 3.0)
+
+
+def test_second_derivatives_are_refused(dev):
+    x, tokens = _logits(3, 50, 17)
+    leaf = x.to(dev).requires_grad_()
+    s = g.token_logprobs(leaf, tokens.to(dev))
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(s.logprob.sum(), leaf, create_graph=True)
