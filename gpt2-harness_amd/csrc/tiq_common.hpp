@@ -104,6 +104,63 @@ __device__ __forceinline__ int code_of(float w, float s, float qmin, float qmax)
     return (int)r;
 }
 
+// max over each 16-lane row of the wavefront, in every lane of the row
+// (DPP moves: pairs, quads, half rows, rows). All 64 lanes must be active.
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t x, uint32_t keep) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)keep, (int)x, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ __forceinline__ uint32_t row16_max_u32(uint32_t v) {
+    v = umax(v, dpp_u32<0xB1>(v, 0u));   // quad_perm [1, 0, 3, 2]
+    v = umax(v, dpp_u32<0x4E>(v, 0u));   // quad_perm [2, 3, 0, 1]
+    v = umax(v, dpp_u32<0x141>(v, 0u));  // row_half_mirror
+    v = umax(v, dpp_u32<0x140>(v, 0u));  // row_mirror
+    return v;
+}
+
+// v_cvt_i32_f32: round-toward-zero conversion that saturates out-of-range
+// values and maps NaN to 0 (defined for every input, unlike a C++ cast).
+__device__ __forceinline__ int cvt_i32_sat(float f) {
+    int r;
+    asm("v_cvt_i32_f32 %0, %1" : "=v"(r) : "v"(f));
+    return r;
+}
+
+
+// Codes of four values, clamp(rint(w / s), qmin, qmax) with w / s the
+// correctly rounded quotient, computed as rint(w * inv), inv = 1 / s
+// correctly rounded. For |w / s| <= 130 the exact product w * inv is within
+// 130 * 2^-23 < 2^-15.9 of the rounded quotient and its own rounding within
+// 2^-17, so the rounded product and the quotient round to the same integer
+// unless w * inv lies within 2^-14 of a half-integer. Beyond 130 a wrong
+// neighbour would still clamp to the same end (qmax <= 127, qmin >= -128),
+// and past 2^23 both are the same integer. Only groups of four with a value
+// near a half-integer (about one in 2000) take the exact division, so the
+// codes equal the per-element division's. Infinite and NaN products give
+// the quotient's codes through the saturating conversion (inf -> the clamp
+// end, NaN -> 0), whichever branch they take.
+__device__ __forceinline__ void codes4(const float4& v, float s, float inv, int qmin, int qmax, int (&c)[4]) {
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    float t[4], e[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        t[k] = __builtin_rintf(x[k] * inv);
+        e[k] = fabsf(fabsf(__builtin_fmaf(x[k], inv, -t[k])) - 0.5f);  // exact w*inv - t, rounded once
+    }
+    const float emin = fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
+    if (!(emin > 0x1p-14f)) {
+        asm volatile("");  // a real branch: the divisions run only in waves that need them
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = __builtin_rintf(x[k] / s);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int q = max(cvt_i32_sat(t[k]), qmin);
+        c[k] = min(q, qmax);
+    }
+}
+
 // fp32 -> bf16 bits, round to nearest even (NaN kept quiet).
 __device__ __forceinline__ uint16_t f32_to_bf16_bits(float f) {
     uint32_t u = __float_as_uint(f);

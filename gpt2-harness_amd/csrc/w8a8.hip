@@ -14,6 +14,7 @@
 // tiles and weight rows to whole tiles, so odd sizes cost no other path; token
 // rows past M are whatever the workspace holds (their outputs are not stored).
 #include <algorithm>
+#include <cstdlib>
 
 #include "tiq_internal.hpp"
 
@@ -60,6 +61,85 @@ __global__ __launch_bounds__(256) void tokens_generic(const TX* __restrict__ x, 
         const float t = __builtin_rintf(v / s);
         const int code = t != t ? 0 : (int)fminf(fmaxf(t, -128.f), 127.f);
         q[TILES ? tile_byte(row, c, U) : row * ldq + c] = (int8_t)code;
+    }
+}
+
+// 16 bytes of a row at any alignment of its elements.
+struct __attribute__((packed, aligned(4))) Bytes16F {
+    float v[4];
+};
+struct __attribute__((packed, aligned(2))) Bytes16H {
+    uint16_t v[8];
+};
+__device__ __forceinline__ void load_16(const float* p, float (&v)[4]) {
+    const Bytes16F t = *reinterpret_cast<const Bytes16F*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = t.v[i];
+}
+__device__ __forceinline__ void load_16(const uint16_t* p, float (&v)[8]) {
+    const Bytes16H t = *reinterpret_cast<const Bytes16H*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = bf16_bits_to_f32(t.v[i]);
+}
+
+// Four rows a workgroup, held in registers: 16 lanes of each wavefront on every row, so a
+// load instruction reads 256 consecutive bytes of each and a store covers 64-byte pieces
+// of the tiles. IT passes of TH / 4 lanes x 16 bytes a row; K >= 16 bytes of elements.
+template <bool TILES, int IT, int TH, typename TX>
+__global__ __launch_bounds__(TH) void tokens_kernel(const TX* __restrict__ x, int64_t ldx, int M, int K,
+                                                    int8_t* __restrict__ q, int64_t ldq, int64_t U,
+                                                    float* __restrict__ scale) {
+    constexpr int VEC = 16 / (int)sizeof(TX), W = TH / 64, STEP = TH / 4 * VEC;
+    __shared__ uint32_t red[W][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (lane >> 4);
+    const int c0 = (wave * 16 + (lane & 15)) * VEC;
+    const TX* xr = x + min(row, (int64_t)M - 1) * ldx;
+    float v[IT][VEC];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) load_16(xr + min(c0 + STEP * i, K - VEC), v[i]);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = c0 + STEP * i;
+        if (c > K - VEC) {  // past the row's last whole piece: its elements one by one
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[i][e] = c + e < K ? load_x(xr + c + e) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) m = umax(m, abs_bits(v[i][e]));
+    }
+    m = row16_max_u32(m);
+    if ((lane & 15) == 0) red[wave][lane >> 4] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = umax(m, red[w][lane >> 4]);
+    if (row >= M) return;
+    const float s = scale_from_amax(__uint_as_float(m), 127.f), inv = 1.0f / s;
+    if (c0 == 0) scale[row] = s;
+    const int end = TILES ? (int)(32 * U) : K;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int c = c0 + STEP * i;
+        if (c >= end) break;
+        uint32_t w[VEC / 4];
+#pragma unroll
+        for (int g = 0; g < VEC / 4; ++g) {
+            int k[4];
+            codes4(make_float4(v[i][4 * g], v[i][4 * g + 1], v[i][4 * g + 2], v[i][4 * g + 3]), s, inv, -128, 127, k);
+            w[g] = (uint32_t)(k[0] & 0xff) | (uint32_t)(k[1] & 0xff) << 8 | (uint32_t)(k[2] & 0xff) << 16 |
+                   (uint32_t)(k[3] & 0xff) << 24;
+        }
+        int8_t* dst = q + (TILES ? tile_byte(row, c, U) : row * ldq + c);
+        if (TILES || (c + VEC <= K && ((uintptr_t)dst & 3) == 0)) {
+            if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+            else if constexpr (TILES) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+            else reinterpret_cast<uint32_t*>(dst)[0] = w[0], reinterpret_cast<uint32_t*>(dst)[1] = w[1];
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (c + e < K) dst[e] = (int8_t)(w[e >> 2] >> 8 * (e & 3));
+        }
     }
 }
 
@@ -129,11 +209,232 @@ __global__ __launch_bounds__(64 * W) void w8a8_direct(const int8_t* __restrict__
     }
 }
 
+// Tile index -> tile: eight contiguous ranges, one an XCD (workgroups go round the XCDs),
+// each walked in groups of four row tiles, so that the workgroups of an XCD that run
+// together share rows and weights in its L2.
+__device__ __forceinline__ void tile_of(int i, int tiles_m, int tiles_n, int& tm, int& tn) {
+    constexpr int XCDS = 8, G = 4;
+    const int total = tiles_m * tiles_n, q = total / XCDS, r = total % XCDS;
+    const int xcd = i % XCDS, local = i / XCDS;
+    const int id = min(xcd, r) * (q + 1) + max(xcd - r, 0) * q + local;
+    const int group = id / (G * tiles_n), in = id % (G * tiles_n);
+    const int gm = min(tiles_m - group * G, G);
+    tm = group * G + in % gm;
+    tn = in / gm;
+}
+
+// The product of many rows. A workgroup of four wavefronts side by side along N owns
+// 32 TM rows x 128 TN columns, a wavefront all the rows and 32 TN columns. The rows' tiles
+// pass through LDS (double buffered, one barrier a k64 step; loaded D - 1 steps before
+// their LDS store), as all four wavefronts need them; the weights' go straight from
+// memory into the registers of the one wavefront that needs them, one and a half steps
+// ahead: 1 KB of consecutive memory an instruction either way, no bank conflicts, no
+// swizzle. Beside each MFMA goes one of the step's other operations.
+template <int TM, int TN, int D, int OCC, typename TY>
+__global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict__ xt, const float* __restrict__ sx,
+                                                        const int8_t* __restrict__ wt, const float* __restrict__ sw,
+                                                        const float* __restrict__ bias, TY* __restrict__ y, int64_t ldy,
+                                                        int M, int N, int U, int tiles_m, int tiles_n) {
+    constexpr int STAGE = TM * 2048;             // bytes of a k64 step of rows
+    constexpr int XL = STAGE / (256 * 16);       // staging loads a thread and step
+    constexpr int NMF = TM * TN;                 // MFMAs a k32 block
+    static_assert(STAGE % 4096 == 0, "whole loads a thread");
+    __shared__ __attribute__((aligned(1024))) int8_t smem[2 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int T = (M + 31) / 32, NT = (N + 31) / 32, nk = U / 2;
+
+    // rows' tile i of the workgroup: 2 KB a step; thread: 16 bytes of tile q (XL of them)
+    const int8_t* xp[XL];
+#pragma unroll
+    for (int q = 0; q < XL; ++q) {
+        const int o = q * 4096 + tid * 16;
+        xp[q] = xt + (int64_t)min(tm * TM + o / 2048, T - 1) * U * 1024 + o % 2048;  // past the last: it again (not stored)
+    }
+    const int8_t* wp[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) wp[j] = wt + (int64_t)min((tn * 4 + wave) * TN + j, NT - 1) * U * 1024 + lane * 16;
+
+    i32x4 st[D][XL], FW[2][2][TN], FX[2][TM];
+    auto gload = [&](int s, int p, int q) { st[p][q] = *reinterpret_cast<const i32x4*>(xp[q] + (int64_t)s * 2048); };
+    auto wload = [&](int s, int p, int kk, int j) {
+        FW[p][kk][j] = *reinterpret_cast<const i32x4*>(wp[j] + (int64_t)s * 2048 + kk * 1024);
+    };
+    auto lstore = [&](int buf, int p, int q) {
+        *reinterpret_cast<i32x4*>(smem + buf * STAGE + q * 4096 + tid * 16) = st[p][q];
+    };
+    auto fread = [&](int buf, int kk, int set, int i) {
+        FX[set][i] = *reinterpret_cast<const i32x4*>(smem + buf * STAGE + i * 2048 + kk * 1024 + lane * 16);
+    };
+    i32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = i32x16{};
+    auto mfma = [&](int set, int p, int kk, int t) {
+        const int i = t / TN, j = t % TN;
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(FX[set][i], FW[p][kk][j], acc[i][j], 0, 0, 0);
+    };
+
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int q = 0; q < XL; ++q) gload(min(d, nk - 1), d, q);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) wload(0, 0, kk, j);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) wload(min(1, nk - 1), 1, 0, j);
+#pragma unroll
+    for (int q = 0; q < XL; ++q) lstore(0, 0, q);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fread(0, 0, 0, i);
+
+    // Step s (staging set p = s % D, weight set w = s % 2): the first k32 block's MFMAs
+    // beside the second's row fragments, stage s + 1's LDS stores and its second
+    // block's weights; the barrier; the second block's beside the next step's first row
+    // fragments, stage s + D's loads and the first block's weights of s + 2. Past the
+    // last stage the loads repeat it.
+    auto step = [&](int s, int p, int w) {
+        const int cur = s & 1, nxt = cur ^ 1, pn = (p + 1) % D;
+        const int s1 = min(s + 1, nk - 1), s2 = min(s + 2, nk - 1), sd = min(s + D, nk - 1);
+        constexpr int NOP = XL + TM + TN;
+        // (the LDS stores first: done by the barrier)
+#pragma unroll
+        for (int t = 0; t < NMF; ++t) {
+            mfma(0, w, 0, t);
+#pragma unroll
+            for (int k = t * NOP / NMF; k < (t + 1) * NOP / NMF; ++k) {
+                if (k < XL) lstore(nxt, pn, k);
+                else if (k < XL + TM) fread(cur, 1, 1, k - XL);
+                else wload(s1, w ^ 1, 1, k - XL - TM);
+            }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NMF; ++t) {
+            mfma(1, w, 1, t);
+#pragma unroll
+            for (int k = t * NOP / NMF; k < (t + 1) * NOP / NMF; ++k) {
+                if (k < TM) fread(nxt, 0, 0, k);
+                else if (k < TM + XL) gload(sd, p, k - TM);
+                else wload(s2, w, 0, k - TM - XL);
+            }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    constexpr int P = D % 2 ? 2 * D : D;  // steps until both sets come round
+    if ((tn * 4 + wave) * TN >= NT) {  // columns past the last: only its share of the staging
+        int s = 0;
+        for (; s < nk; s += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                if (s + d >= nk) break;
+#pragma unroll
+                for (int q = 0; q < XL; ++q) lstore((s + d + 1) & 1, (d + 1) % D, q);
+                __syncthreads();
+#pragma unroll
+                for (int q = 0; q < XL; ++q) gload(min(s + d + D, nk - 1), d, q);
+            }
+        }
+        return;
+    }
+    int s = 0;
+    for (; s + P <= nk; s += P) {
+#pragma unroll
+        for (int d = 0; d < P; ++d) step(s + d, d % D, d % 2);
+    }
+#pragma unroll
+    for (int d = 0; d < P - 1; ++d)
+        if (s + d < nk) step(s + d, d % D, d % 2);
+
+    // result register q of lane (r, h): row 8 (q / 4) + 4 h + q % 4, column r. The scales
+    // are asked for all at once, whole tiles are stored without a test, and bf16
+    // neighbours of two rows swap a value each, so that a store takes four bytes a lane.
+    const int r = lane & 31, h = lane >> 5;
+    const int m0 = tm * TM * 32 + 4 * h, n0 = (tn * 4 + wave) * TN * 32;
+    float scw[TN], b[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int n = min(n0 + 32 * j + r, N - 1);
+        scw[j] = sw[n];
+        b[j] = bias ? bias[n] : 0.f;
+    }
+    float4 s4[TM][4];  // (the workspace holds whole tiles of scales)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            s4[i][g] = *reinterpret_cast<const float4*>(sx + min(tm * TM + i, T - 1) * 32 + 8 * g + 4 * h);
+    auto value = [&](int i, int j, int g, int e) {
+        const float sxe = e == 0 ? s4[i][g].x : e == 1 ? s4[i][g].y : e == 2 ? s4[i][g].z : s4[i][g].w;
+        return finish(acc[i][j][4 * g + e], sxe, scw[j], b[j]);
+    };
+    const bool whole = (tm + 1) * TM * 32 <= M && n0 + 32 * TN <= N;
+    if (whole && (sizeof(TY) == 4 || (((uintptr_t)y | (uint64_t)ldy * 2) & 3) == 0)) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                TY* dst = y + (int64_t)(m0 + 32 * i + 8 * g) * ldy + n0 + r;
+                if constexpr (sizeof(TY) == 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) dst[(int64_t)e * ldy + 32 * j] = value(i, j, g, e);
+                } else {
+                    const bool odd = r & 1;  // even lanes store row e, odd ones row e + 1
+                    dst += odd ? ldy - 1 : 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) {
+                            const float v0 = value(i, j, g, e), v1 = value(i, j, g, e + 1);
+                            const float got = dpp_move<0xB1>(odd ? v0 : v1);
+                            *reinterpret_cast<uint32_t*>(dst + (int64_t)e * ldy + 32 * j) =
+                                odd ? pk_bf16(got, v1) : pk_bf16(v0, got);
+                        }
+                }
+            }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int m = m0 + 32 * i + 8 * g + e;
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    if (m < M && n0 + 32 * j + r < N) store_y(y + (int64_t)m * ldy + n0 + 32 * j + r, value(i, j, g, e));
+            }
+}
+
 size_t round256(size_t b) { return (b + 255) / 256 * 256; }
 
 template <bool TILES, typename TX>
 int launch_tokens(const TX* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                   hipStream_t st) {
+    constexpr int VEC = 16 / (int)sizeof(TX);
+    auto held = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + 3) / 4)), dim3(threads), 0, st, x, ldx, (int)rows, (int)K,
+                           q, ldq, units_of(K), scale);
+        return launch_status();
+    };
+    // passes over the columns a row has, with its padding
+    const int64_t cols = TILES ? 32 * units_of(K) : K, small = (cols + 64 * VEC - 1) / (64 * VEC);
+    if (K >= VEC && small <= 2) return held(tokens_kernel<TILES, 2, 256, TX>, 256);
+    if (K >= VEC && small <= 4) return held(tokens_kernel<TILES, 4, 256, TX>, 256);
+    if (K >= VEC && small <= 8) return held(tokens_kernel<TILES, 8, 256, TX>, 256);
+    if (K >= VEC && small <= 16) return held(tokens_kernel<TILES, 4, 1024, TX>, 1024);
+    if (K >= VEC && small <= 32) return held(tokens_kernel<TILES, 8, 1024, TX>, 1024);
     hipLaunchKernelGGL((tokens_generic<TILES, TX>), dim3((unsigned)rows), dim3(256), 0, st, x, ldx, K, q, ldq,
                        units_of(K), scale);
     return launch_status();
@@ -147,6 +448,25 @@ int run_w8a8(const TX* x, int64_t M, int64_t K, int64_t ldx, const int8_t* wt, c
     float* sx = reinterpret_cast<float*>(ws + tiles_of(M) * U * 1024);
     const int rc = launch_tokens<true>(x, M, K, ldx, xt, (int64_t)0, sx, st);
     if (rc != TIQ_OK) return rc;
+    if (const char* e = getenv("WS")) {
+        const int TM = atoi(e) / 10, TNN = atoi(e) % 10;
+        const int tm = (int)((tiles_of(M) + TM - 1) / TM), tn = (int)((TN + 4 * TNN - 1) / (4 * TNN));
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(tm * tn), dim3(256), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M, (int)N,
+                               (int)U, tm, tn);
+            return launch_status();
+        };
+        switch (TM * 10 + TNN) {
+            case 42: return go(w8a8_staged<4, 2, 3, 2, TY>);
+            case 41: return go(w8a8_staged<4, 1, 3, 2, TY>);
+            case 22: return go(w8a8_staged<2, 2, 4, 2, TY>);
+            case 21: return go(w8a8_staged<2, 1, 4, 2, TY>);
+            case 82: return go(w8a8_staged<8, 2, 3, 1, TY>);
+            case 44: return go(w8a8_staged<4, 4, 3, 1, TY>);
+            case 43: return go(w8a8_staged<4, 3, 3, 1, TY>);
+            case 62: return go(w8a8_staged<6, 2, 3, 1, TY>);
+        }
+    }
     hipLaunchKernelGGL((w8a8_direct<4, TY>), dim3((unsigned)(tiles_of(M) * TN)), dim3(256), 0, st, xt, sx, wt, sw,
                        bias, y, ldy, (int)M, (int)N, (int)U, (int)TN);
     return launch_status();
@@ -199,7 +519,7 @@ extern "C" int tiq_w8a8_untile(const int8_t* tiles, int64_t N, int64_t K, int8_t
 
 extern "C" size_t tiq_linear_w8a8_workspace(int64_t M, int64_t K, int64_t N) {
     if (M <= 0 || K <= 0 || N <= 0) return 0;
-    return round256((size_t)(tiles_of(M) * units_of(K) * 1024 + 4 * M));
+    return round256((size_t)(tiles_of(M) * (units_of(K) * 1024 + 128)));  // (scales of whole tiles)
 }
 
 extern "C" int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const int8_t* w_tiles,
