@@ -174,37 +174,168 @@ __device__ __forceinline__ float finish(int sum, float sx, float sw, float b) {
     return fmaf((float)sum * sx, sw, b);
 }
 
-// The product without a staging step: W wavefronts share the K range of one 32 x 32
-// output tile, each with its own operand loads (1 KB of consecutive memory an
-// instruction), and add their sums through LDS.
+// The row's scale and codes in LDS for a product of few rows (M <= kFusedRows): W wavefronts,
+// W / Mp of them a row (Mp: M's next power of two), K <= kFusedK columns, the padding
+// columns zero. Row m's codes lie at m * 32 U.
+constexpr int kFusedRows = 4, kFusedK = 8192;
+template <int W, typename TX>
+__device__ __forceinline__ void quantize_rows(const TX* __restrict__ x, int64_t ldx, int M, int K, int end,
+                                              int8_t* __restrict__ codes, float* __restrict__ scale,
+                                              uint32_t* __restrict__ red) {
+    constexpr int VEC = 16 / (int)sizeof(TX);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int Mp = M <= 1 ? 1 : M <= 2 ? 2 : 4, per = W / Mp;  // wavefronts a row
+    const int row = wave / per, c0 = ((wave - row * per) * 64 + lane) * VEC, step = per * 64 * VEC;
+    const TX* xr = x + (int64_t)min(row, M - 1) * ldx;
+    // `f` over the row's 16-byte pieces, past its end zeros
+    auto pieces = [&](auto f) {
+        for (int c = c0; c < end; c += 4 * step) {
+            float v[4][VEC];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_16(xr + min(c + step * i, K - VEC), v[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int ci = c + step * i;
+                if (ci >= end) break;
+                if (ci > K - VEC) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) v[i][e] = ci + e < K ? load_x(xr + ci + e) : 0.f;
+                }
+                f(ci, v[i]);
+            }
+        }
+    };
+    uint32_t m = 0;
+    pieces([&](int, const float(&v)[VEC]) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) m = umax(m, abs_bits(v[e]));
+    });
+    m = wave_max_u32(m);
+    if (lane == 0) red[wave] = m;
+    __syncthreads();
+    for (int w = 0; w < per; ++w) m = umax(m, red[row * per + w]);
+    const float s = scale_from_amax(__uint_as_float(m), 127.f), inv = 1.0f / s;
+    if (wave == row * per && lane == 0) scale[row] = s;
+    pieces([&](int c, const float(&v)[VEC]) {
+#pragma unroll
+        for (int g = 0; g < VEC / 4; ++g) {
+            int k[4];
+            codes4(make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]), s, inv, -128, 127, k);
+            *reinterpret_cast<uint32_t*>(codes + row * end + c + 4 * g) =
+                (uint32_t)(k[0] & 0xff) | (uint32_t)(k[1] & 0xff) << 8 | (uint32_t)(k[2] & 0xff) << 16 |
+                (uint32_t)(k[3] & 0xff) << 24;
+        }
+    });
+}
+
+// The product of up to 16 rows: a workgroup of W wavefronts per 16 output columns, the K
+// range dealt out to them in k64 blocks, their sums added through LDS. The weights are
+// read once, by the wavefront that multiplies them, PF blocks on their way at a time.
+// FUSE (few rows): the workgroup quantizes the rows itself, behind the first weights'
+// loads, which spares a launch; else their tiles come from tokens_kernel.
+template <int W, bool FUSE, typename TX, typename TY>
+__global__ __launch_bounds__(64 * W) void w8a8_small(const TX* __restrict__ x, int64_t ldx,
+                                                     const int8_t* __restrict__ xt, const float* __restrict__ sx,
+                                                     const int8_t* __restrict__ wt, const float* __restrict__ sw,
+                                                     const float* __restrict__ bias, TY* __restrict__ y, int64_t ldy,
+                                                     int M, int N, int K, int U) {
+    constexpr int PF = 4;
+    __shared__ int part[W][256];
+    __shared__ float scale[FUSE ? kFusedRows : 1];
+    __shared__ uint32_t red[W];
+    extern __shared__ __attribute__((aligned(16))) int8_t codes[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, c = lane >> 4, tn = blockIdx.x;
+    const int nb = U / 2;  // k64 blocks; this wavefront's: wave, wave + W, ...
+    const int place = (c >> 1) * 1024 + (c & 1) * 512 + r * 16;
+    const int8_t* wp = wt + (int64_t)(tn >> 1) * U * 1024 + (tn & 1) * 256 + place;
+    const int8_t* xp = FUSE ? nullptr : xt + place;
+    i32x4 fw[PF], fx[PF];
+    auto load = [&](int b0) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            const int b = min(b0 + W * i, nb - 1);
+            fw[i] = *reinterpret_cast<const i32x4*>(wp + (int64_t)b * 2048);
+            if constexpr (!FUSE) fx[i] = *reinterpret_cast<const i32x4*>(xp + (int64_t)b * 2048);
+        }
+    };
+    load(wave);
+    if constexpr (FUSE) {
+        quantize_rows<W>(x, ldx, M, K, 32 * U, codes, scale, red);
+        __syncthreads();
+    }
+    i32x4 acc = {};
+    for (int b0 = wave; b0 < nb; b0 += W * PF) {
+        i32x4 w[PF], a[PF];
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            w[i] = fw[i];
+            if constexpr (FUSE)
+                a[i] = *reinterpret_cast<const i32x4*>(codes + min(r, M - 1) * 32 * U + min(b0 + W * i, nb - 1) * 64 + 16 * c);
+            else a[i] = fx[i];
+        }
+        if (b0 + W * PF < nb) load(b0 + W * PF);
+#pragma unroll
+        for (int i = 0; i < PF; ++i)
+            if (b0 + W * i < nb) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], w[i], acc, 0, 0, 0);
+    }
+    // result register q of lane (r, c): row 4 c + q, column r
+#pragma unroll
+    for (int q = 0; q < 4; ++q) part[wave][(4 * c + q) * 16 + r] = acc[q];
+    __syncthreads();
+    const int m = tid >> 4, n = 16 * tn + (tid & 15);
+    if (tid >= 256 || m >= M || n >= N) return;
+    int s = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += part[w][tid];
+    store_y(y + (int64_t)m * ldy + n, finish(s, FUSE ? scale[m] : sx[m], sw[n], bias ? bias[n] : 0.f));
+}
+
+// The product without a staging step: W wavefronts share the K range of a 32 x 32 output
+// tile, each with its own operand loads, PF units on their way at a time, and add
+// their sums through LDS.
 template <int W, typename TY>
 __global__ __launch_bounds__(64 * W) void w8a8_direct(const int8_t* __restrict__ xt, const float* __restrict__ sx,
                                                       const int8_t* __restrict__ wt, const float* __restrict__ sw,
                                                       const float* __restrict__ bias, TY* __restrict__ y, int64_t ldy,
-                                                      int M, int N, int U, int tiles_n) {
-    constexpr int LD = 36;  // a row of sums in LDS, padded to whole 16-byte chunks
-    __shared__ __attribute__((aligned(16))) int part[W][32 * LD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+                                                      int M, int N, int U, int tiles_m) {
+    constexpr int PF = 4;
+    __shared__ int part[W][32 * 33];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 31, h = lane >> 5;
-    const int tm = blockIdx.x / tiles_n, tn = blockIdx.x % tiles_n;
+    const int tm = blockIdx.x % tiles_m, tn = blockIdx.x / tiles_m;  // a weight tile's workgroups side by side
     const int8_t* xp = xt + (int64_t)tm * U * 1024 + lane * 16;
     const int8_t* wp = wt + (int64_t)tn * U * 1024 + lane * 16;
+    i32x4 fa[PF], fb[PF];
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            const int u = min(u0 + W * i, U - 1);
+            fa[i] = *reinterpret_cast<const i32x4*>(xp + (int64_t)u * 1024);
+            fb[i] = *reinterpret_cast<const i32x4*>(wp + (int64_t)u * 1024);
+        }
+    };
+    load(wave);
     i32x16 acc = {};
-    for (int u = wave; u < U; u += W) {
-        const i32x4 a = *reinterpret_cast<const i32x4*>(xp + u * 1024);
-        const i32x4 b = *reinterpret_cast<const i32x4*>(wp + u * 1024);
-        acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, acc, 0, 0, 0);
+    for (int u0 = wave; u0 < U; u0 += W * PF) {
+        i32x4 a[PF], b[PF];
+#pragma unroll
+        for (int i = 0; i < PF; ++i) a[i] = fa[i], b[i] = fb[i];
+        if (u0 + W * PF < U) load(u0 + W * PF);
+#pragma unroll
+        for (int i = 0; i < PF; ++i)
+            if (u0 + W * i < U) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[i], acc, 0, 0, 0);
     }
     // result register q of lane (r, h): row 8 (q / 4) + 4 h + q % 4, column r
 #pragma unroll
-    for (int q = 0; q < 16; ++q) part[wave][(8 * (q >> 2) + 4 * h + (q & 3)) * LD + r] = acc[q];
+    for (int q = 0; q < 16; ++q) part[wave][(8 * (q >> 2) + 4 * h + (q & 3)) * 33 + r] = acc[q];
     __syncthreads();
     for (int i = threadIdx.x; i < 1024; i += 64 * W) {
         const int m = 32 * tm + (i >> 5), n = 32 * tn + (i & 31);
         if (m >= M || n >= N) continue;
         int s = 0;
 #pragma unroll
-        for (int w = 0; w < W; ++w) s += part[w][(i >> 5) * LD + (i & 31)];
+        for (int w = 0; w < W; ++w) s += part[w][(i >> 5) * 33 + (i & 31)];
         store_y(y + (int64_t)m * ldy + n, finish(s, sx[m], sw[n], bias ? bias[n] : 0.f));
     }
 }
@@ -440,36 +571,59 @@ int launch_tokens(const TX* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, 
     return launch_status();
 }
 
+// How a product of M rows is taken.
+enum Path : int { kSmall, kDirect, kStaged };
+
 template <typename TX, typename TY>
 int run_w8a8(const TX* x, int64_t M, int64_t K, int64_t ldx, const int8_t* wt, const float* sw, const float* bias,
              int64_t N, TY* y, int64_t ldy, uint8_t* ws, hipStream_t st) {
-    const int64_t U = units_of(K), TN = tiles_of(N);
+    const int64_t U = units_of(K), T = tiles_of(M), NT = tiles_of(N);
     int8_t* xt = reinterpret_cast<int8_t*>(ws);
-    float* sx = reinterpret_cast<float*>(ws + tiles_of(M) * U * 1024);
+    float* sx = reinterpret_cast<float*>(ws + T * U * 1024);
+    const char* e = getenv("WS");
+    const int force = e ? atoi(e) : 0;
+    const bool fuse = M <= kFusedRows && K <= kFusedK && K >= 16 / (int)sizeof(TX) && force != 1;
+    if (M <= 16 && force < 2 && fuse) {
+        auto go = [&](auto kernel, int W) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((N + 15) / 16)), dim3(64 * W), (size_t)(M * 32 * U), st, x, ldx, xt,
+                               sx, wt, sw, bias, y, ldy, (int)M, (int)N, (int)K, (int)U);
+            return launch_status();
+        };
+        return K > 2048 ? go(w8a8_small<16, true, TX, TY>, 16) : go(w8a8_small<8, true, TX, TY>, 8);
+    }
     const int rc = launch_tokens<true>(x, M, K, ldx, xt, (int64_t)0, sx, st);
     if (rc != TIQ_OK) return rc;
-    if (const char* e = getenv("WS")) {
-        const int TM = atoi(e) / 10, TNN = atoi(e) % 10;
-        const int tm = (int)((tiles_of(M) + TM - 1) / TM), tn = (int)((TN + 4 * TNN - 1) / (4 * TNN));
+    if (M <= 16 && force < 2) {
+        auto go = [&](auto kernel, int W) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((N + 15) / 16)), dim3(64 * W), 0, st, x, ldx, xt, sx, wt, sw, bias,
+                               y, ldy, (int)M, (int)N, (int)K, (int)U);
+            return launch_status();
+        };
+        return K > 2048 ? go(w8a8_small<16, false, TX, TY>, 16) : go(w8a8_small<8, false, TX, TY>, 8);
+    }
+    if (force > 9) {
+        const int TM = force / 10, TNN = force % 10;
+        const int tm = (int)((T + TM - 1) / TM), tn = (int)((NT + 4 * TNN - 1) / (4 * TNN));
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(tm * tn), dim3(256), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M, (int)N,
                                (int)U, tm, tn);
             return launch_status();
         };
-        switch (TM * 10 + TNN) {
+        switch (force) {
             case 42: return go(w8a8_staged<4, 2, 3, 2, TY>);
             case 41: return go(w8a8_staged<4, 1, 3, 2, TY>);
             case 22: return go(w8a8_staged<2, 2, 4, 2, TY>);
             case 21: return go(w8a8_staged<2, 1, 4, 2, TY>);
-            case 82: return go(w8a8_staged<8, 2, 3, 1, TY>);
-            case 44: return go(w8a8_staged<4, 4, 3, 1, TY>);
-            case 43: return go(w8a8_staged<4, 3, 3, 1, TY>);
-            case 62: return go(w8a8_staged<6, 2, 3, 1, TY>);
         }
     }
-    hipLaunchKernelGGL((w8a8_direct<4, TY>), dim3((unsigned)(tiles_of(M) * TN)), dim3(256), 0, st, xt, sx, wt, sw,
-                       bias, y, ldy, (int)M, (int)N, (int)U, (int)TN);
-    return launch_status();
+    auto go = [&](auto kernel, int W) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(T * NT)), dim3(64 * W), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
+                           (int)N, (int)U, (int)T);
+        return launch_status();
+    };
+    if (force == 4) return go(w8a8_direct<4, TY>, 4);
+    if (force == 8) return go(w8a8_direct<8, TY>, 8);
+    return K > 2048 ? go(w8a8_direct<8, TY>, 8) : go(w8a8_direct<4, TY>, 4);
 }
 
 bool known_dtype(int d) { return d == TIQ_F32 || d == TIQ_BF16; }
