@@ -14,7 +14,6 @@
 // tiles and weight rows to whole tiles, so odd sizes cost no other path; token
 // rows past M are whatever the workspace holds (their outputs are not stored).
 #include <algorithm>
-#include <cstdlib>
 
 #include "tiq_internal.hpp"
 
@@ -291,53 +290,81 @@ __global__ __launch_bounds__(64 * W) void w8a8_small(const TX* __restrict__ x, i
     store_y(y + (int64_t)m * ldy + n, finish(s, FUSE ? scale[m] : sx[m], sw[n], bias ? bias[n] : 0.f));
 }
 
-// The product without a staging step: W wavefronts share the K range of a 32 x 32 output
-// tile, each with its own operand loads, PF units on their way at a time, and add
-// their sums through LDS.
-template <int W, typename TY>
+// The product without a staging step: W wavefronts share the K range of an output tile of
+// TM x TN 32 x 32 tiles, each with its own operand loads, PF units on their way at a
+// time, and add their sums through LDS, a 32 x 32 tile after the other.
+template <int W, int TM, int TN, int PF, typename TY>
 __global__ __launch_bounds__(64 * W) void w8a8_direct(const int8_t* __restrict__ xt, const float* __restrict__ sx,
                                                       const int8_t* __restrict__ wt, const float* __restrict__ sw,
                                                       const float* __restrict__ bias, TY* __restrict__ y, int64_t ldy,
                                                       int M, int N, int U, int tiles_m) {
-    constexpr int PF = 4;
-    __shared__ int part[W][32 * 33];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int G = TM * TN > 1 ? 2 : 1;  // sets of sums in LDS: one barrier a tile
+    __shared__ int part[G][W][32 * 33];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
     const int tm = blockIdx.x % tiles_m, tn = blockIdx.x / tiles_m;  // a weight tile's workgroups side by side
-    const int8_t* xp = xt + (int64_t)tm * U * 1024 + lane * 16;
-    const int8_t* wp = wt + (int64_t)tn * U * 1024 + lane * 16;
-    i32x4 fa[PF], fb[PF];
+    const int T = (M + 31) / 32, NT = (N + 31) / 32;
+    const int8_t *xp[TM], *wp[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xp[i] = xt + (int64_t)min(tm * TM + i, T - 1) * U * 1024 + lane * 16;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) wp[j] = wt + (int64_t)min(tn * TN + j, NT - 1) * U * 1024 + lane * 16;
+    i32x4 fa[PF][TM], fb[PF][TN];
     auto load = [&](int u0) {
 #pragma unroll
-        for (int i = 0; i < PF; ++i) {
-            const int u = min(u0 + W * i, U - 1);
-            fa[i] = *reinterpret_cast<const i32x4*>(xp + (int64_t)u * 1024);
-            fb[i] = *reinterpret_cast<const i32x4*>(wp + (int64_t)u * 1024);
+        for (int p = 0; p < PF; ++p) {
+            const int64_t o = (int64_t)min(u0 + W * p, U - 1) * 1024;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[p][i] = *reinterpret_cast<const i32x4*>(xp[i] + o);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[p][j] = *reinterpret_cast<const i32x4*>(wp[j] + o);
         }
     };
     load(wave);
-    i32x16 acc = {};
-    for (int u0 = wave; u0 < U; u0 += W * PF) {
-        i32x4 a[PF], b[PF];
+    i32x16 acc[TM][TN];
 #pragma unroll
-        for (int i = 0; i < PF; ++i) a[i] = fa[i], b[i] = fb[i];
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = i32x16{};
+    for (int u0 = wave; u0 < U; u0 += W * PF) {
+        i32x4 a[PF][TM], b[PF][TN];
+#pragma unroll
+        for (int p = 0; p < PF; ++p) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) a[p][i] = fa[p][i];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) b[p][j] = fb[p][j];
+        }
         if (u0 + W * PF < U) load(u0 + W * PF);
 #pragma unroll
-        for (int i = 0; i < PF; ++i)
-            if (u0 + W * i < U) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[i], acc, 0, 0, 0);
+        for (int p = 0; p < PF; ++p) {
+            if (u0 + W * p >= U) break;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[p][i], b[p][j], acc[i][j], 0, 0, 0);
+        }
     }
     // result register q of lane (r, h): row 8 (q / 4) + 4 h + q % 4, column r
 #pragma unroll
-    for (int q = 0; q < 16; ++q) part[wave][(8 * (q >> 2) + 4 * h + (q & 3)) * 33 + r] = acc[q];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 1024; i += 64 * W) {
-        const int m = 32 * tm + (i >> 5), n = 32 * tn + (i & 31);
-        if (m >= M || n >= N) continue;
-        int s = 0;
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int w = 0; w < W; ++w) s += part[w][(i >> 5) * 33 + (i & 31)];
-        store_y(y + (int64_t)m * ldy + n, finish(s, sx[m], sw[n], bias ? bias[n] : 0.f));
-    }
+        for (int j = 0; j < TN; ++j) {
+            int(&set)[W][32 * 33] = part[(i * TN + j) % G];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) set[wave][(8 * (q >> 2) + 4 * h + (q & 3)) * 33 + r] = acc[i][j][q];
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 1024 / (64 * W); ++e) {
+                const int o = tid + 64 * W * e;
+                const int m = 32 * (tm * TM + i) + (o >> 5), n = 32 * (tn * TN + j) + (o & 31);
+                int s = 0;
+#pragma unroll
+                for (int w = 0; w < W; ++w) s += set[w][(o >> 5) * 33 + (o & 31)];
+                if (m < M && n < N) store_y(y + (int64_t)m * ldy + n, finish(s, sx[m], sw[n], bias ? bias[n] : 0.f));
+            }
+        }
 }
 
 // Tile index -> tile: eight contiguous ranges, one an XCD (workgroups go round the XCDs),
@@ -358,10 +385,9 @@ __device__ __forceinline__ void tile_of(int i, int tiles_m, int tiles_n, int& tm
 // 32 TM rows x 128 TN columns, a wavefront all the rows and 32 TN columns. The rows' tiles
 // pass through LDS (double buffered, one barrier a k64 step; loaded D - 1 steps before
 // their LDS store), as all four wavefronts need them; the weights' go straight from
-// memory into the registers of the one wavefront that needs them, one and a half steps
-// ahead: 1 KB of consecutive memory an instruction either way, no bank conflicts, no
+// memory into the registers of the one wavefront that needs them, WD - 1/2 steps ahead: 1 KB of consecutive memory an instruction either way, no bank conflicts, no
 // swizzle. Beside each MFMA goes one of the step's other operations.
-template <int TM, int TN, int D, int OCC, typename TY>
+template <int TM, int TN, int D, int WD, int OCC, typename TY>
 __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict__ xt, const float* __restrict__ sx,
                                                         const int8_t* __restrict__ wt, const float* __restrict__ sw,
                                                         const float* __restrict__ bias, TY* __restrict__ y, int64_t ldy,
@@ -387,7 +413,7 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
 #pragma unroll
     for (int j = 0; j < TN; ++j) wp[j] = wt + (int64_t)min((tn * 4 + wave) * TN + j, NT - 1) * U * 1024 + lane * 16;
 
-    i32x4 st[D][XL], FW[2][2][TN], FX[2][TM];
+    i32x4 st[D][XL], FW[WD][2][TN], FX[2][TM];
     auto gload = [&](int s, int p, int q) { st[p][q] = *reinterpret_cast<const i32x4*>(xp[q] + (int64_t)s * 2048); };
     auto wload = [&](int s, int p, int kk, int j) {
         FW[p][kk][j] = *reinterpret_cast<const i32x4*>(wp[j] + (int64_t)s * 2048 + kk * 1024);
@@ -413,25 +439,25 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
 #pragma unroll
         for (int q = 0; q < XL; ++q) gload(min(d, nk - 1), d, q);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int d = 0; d < WD; ++d)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) wload(0, 0, kk, j);
+        for (int kk = 0; kk < (d < WD - 1 ? 2 : 1); ++kk)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) wload(min(1, nk - 1), 1, 0, j);
+            for (int j = 0; j < TN; ++j) wload(min(d, nk - 1), d, kk, j);
 #pragma unroll
     for (int q = 0; q < XL; ++q) lstore(0, 0, q);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < TM; ++i) fread(0, 0, 0, i);
 
-    // Step s (staging set p = s % D, weight set w = s % 2): the first k32 block's MFMAs
-    // beside the second's row fragments, stage s + 1's LDS stores and its second
-    // block's weights; the barrier; the second block's beside the next step's first row
-    // fragments, stage s + D's loads and the first block's weights of s + 2. Past the
-    // last stage the loads repeat it.
+    // Step s (staging set p = s % D, weight set w = s % WD): the first k32 block's MFMAs
+    // beside stage s + 1's LDS stores, the second block's row fragments and the
+    // second block's weights of s + WD - 1; the barrier; the second block's beside the
+    // next step's first row fragments, stage s + D's loads and the first block's weights
+    // of s + WD. Past the last stage the loads repeat it.
     auto step = [&](int s, int p, int w) {
         const int cur = s & 1, nxt = cur ^ 1, pn = (p + 1) % D;
-        const int s1 = min(s + 1, nk - 1), s2 = min(s + 2, nk - 1), sd = min(s + D, nk - 1);
+        const int s1 = min(s + WD - 1, nk - 1), s2 = min(s + WD, nk - 1), sd = min(s + D, nk - 1);
         constexpr int NOP = XL + TM + TN;
         // (the LDS stores first: done by the barrier)
 #pragma unroll
@@ -441,7 +467,7 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
             for (int k = t * NOP / NMF; k < (t + 1) * NOP / NMF; ++k) {
                 if (k < XL) lstore(nxt, pn, k);
                 else if (k < XL + TM) fread(cur, 1, 1, k - XL);
-                else wload(s1, w ^ 1, 1, k - XL - TM);
+                else wload(s1, (w + WD - 1) % WD, 1, k - XL - TM);
             }
             asm volatile("" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
@@ -460,7 +486,8 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    constexpr int P = D % 2 ? 2 * D : D;  // steps until both sets come round
+    constexpr int P = D % 2 ? 2 * D : D;  // steps until the sets and the buffers come round
+    static_assert(P % WD == 0, "weight sets");
     if ((tn * 4 + wave) * TN >= NT) {  // columns past the last: only its share of the staging
         int s = 0;
         for (; s < nk; s += D) {
@@ -479,11 +506,11 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
     int s = 0;
     for (; s + P <= nk; s += P) {
 #pragma unroll
-        for (int d = 0; d < P; ++d) step(s + d, d % D, d % 2);
+        for (int d = 0; d < P; ++d) step(s + d, d % D, d % WD);
     }
 #pragma unroll
     for (int d = 0; d < P - 1; ++d)
-        if (s + d < nk) step(s + d, d % D, d % 2);
+        if (s + d < nk) step(s + d, d % D, d % WD);
 
     // result register q of lane (r, h): row 8 (q / 4) + 4 h + q % 4, column r. The scales
     // are asked for all at once, whole tiles are stored without a test, and bf16
@@ -571,8 +598,25 @@ int launch_tokens(const TX* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, 
     return launch_status();
 }
 
-// How a product of M rows is taken.
-enum Path : int { kSmall, kDirect, kStaged };
+// How a product over more than 16 rows is taken, by its 32 x 32 output tiles (rows' T,
+// columns' NT); us with the rows' quantization, fp32, both sides:
+//   few tiles: the direct product, whose wavefronts need no barrier on the way (T NT =
+//     600, 384 x 1600 x 1600: 10.6 against 11.2 .. 12.2 staged; 1600, 1024 x 1600 x 1600:
+//     17.1 against 12.4); 2 x 2 tiles a workgroup where K is long (512 x 6400 x 1600: 22.9
+//     against 28.1);
+//   128 x 256 staged tiles where those are many and K is not short (1024 x 1600 x 4800:
+//     20.2 against 24.9 with 64 x 256; 8192 x 768 x 2304: 37.5 against 33.5);
+//   64 x 256 where those are many (2048 x 1600 x 1600, 224 of them: 17.4 against 18.7 with
+//     64 x 128; 1024 x 1600 x 1600, 112: 13.6 against 12.4), else 64 x 128.
+enum Path { kDirect, kDirectLong, kStaged64x128, kStaged64x256, kStaged128x256 };
+
+Path path_of(int64_t T, int64_t NT, int64_t K) {
+    if (T * NT <= 400) return kDirect;
+    if (K >= 3200 && T * NT <= 1200) return kDirectLong;
+    if (T * NT <= 800) return kDirect;
+    if (K >= 1280 && (T + 3) / 4 * ((NT + 7) / 8) >= 150) return kStaged128x256;
+    return (T + 1) / 2 * ((NT + 7) / 8) >= 150 ? kStaged64x256 : kStaged64x128;
+}
 
 template <typename TX, typename TY>
 int run_w8a8(const TX* x, int64_t M, int64_t K, int64_t ldx, const int8_t* wt, const float* sw, const float* bias,
@@ -580,50 +624,39 @@ int run_w8a8(const TX* x, int64_t M, int64_t K, int64_t ldx, const int8_t* wt, c
     const int64_t U = units_of(K), T = tiles_of(M), NT = tiles_of(N);
     int8_t* xt = reinterpret_cast<int8_t*>(ws);
     float* sx = reinterpret_cast<float*>(ws + T * U * 1024);
-    const char* e = getenv("WS");
-    const int force = e ? atoi(e) : 0;
-    const bool fuse = M <= kFusedRows && K <= kFusedK && K >= 16 / (int)sizeof(TX) && force != 1;
-    if (M <= 16 && force < 2 && fuse) {
-        auto go = [&](auto kernel, int W) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)((N + 15) / 16)), dim3(64 * W), (size_t)(M * 32 * U), st, x, ldx, xt,
-                               sx, wt, sw, bias, y, ldy, (int)M, (int)N, (int)K, (int)U);
-            return launch_status();
-        };
-        return K > 2048 ? go(w8a8_small<16, true, TX, TY>, 16) : go(w8a8_small<8, true, TX, TY>, 8);
+    auto small = [&](auto kernel, int W, size_t lds) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((N + 15) / 16)), dim3(64 * W), lds, st, x, ldx, xt, sx, wt, sw, bias,
+                           y, ldy, (int)M, (int)N, (int)K, (int)U);
+        return launch_status();
+    };
+    // (us in a graph, rows quantized by the workgroups / by a launch before: 1 x 768 x 2304
+    // 3.5 / 5.3, 1 x 6400 x 1600 5.4 / 9.2, 4 x 6400 x 1600 8.0 / 9.1)
+    if (M <= kFusedRows && K <= kFusedK && K >= 16 / (int)sizeof(TX)) {
+        const size_t lds = (size_t)(M * 32 * U);
+        return K > 2048 ? small(w8a8_small<16, true, TX, TY>, 16, lds) : small(w8a8_small<8, true, TX, TY>, 8, lds);
     }
     const int rc = launch_tokens<true>(x, M, K, ldx, xt, (int64_t)0, sx, st);
     if (rc != TIQ_OK) return rc;
-    if (M <= 16 && force < 2) {
-        auto go = [&](auto kernel, int W) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)((N + 15) / 16)), dim3(64 * W), 0, st, x, ldx, xt, sx, wt, sw, bias,
-                               y, ldy, (int)M, (int)N, (int)K, (int)U);
-            return launch_status();
-        };
-        return K > 2048 ? go(w8a8_small<16, false, TX, TY>, 16) : go(w8a8_small<8, false, TX, TY>, 8);
-    }
-    if (force > 9) {
-        const int TM = force / 10, TNN = force % 10;
-        const int tm = (int)((T + TM - 1) / TM), tn = (int)((NT + 4 * TNN - 1) / (4 * TNN));
-        auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(tm * tn), dim3(256), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M, (int)N,
-                               (int)U, tm, tn);
-            return launch_status();
-        };
-        switch (force) {
-            case 42: return go(w8a8_staged<4, 2, 3, 2, TY>);
-            case 41: return go(w8a8_staged<4, 1, 3, 2, TY>);
-            case 22: return go(w8a8_staged<2, 2, 4, 2, TY>);
-            case 21: return go(w8a8_staged<2, 1, 4, 2, TY>);
-        }
-    }
-    auto go = [&](auto kernel, int W) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(T * NT)), dim3(64 * W), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
-                           (int)N, (int)U, (int)T);
+    if (M <= 16) return K > 2048 ? small(w8a8_small<16, false, TX, TY>, 16, 0) : small(w8a8_small<8, false, TX, TY>, 8, 0);
+    auto direct = [&](auto kernel, int TM, int TN) {
+        const int64_t tm = (T + TM - 1) / TM, tn = (NT + TN - 1) / TN;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(512), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
+                           (int)N, (int)U, (int)tm);
         return launch_status();
     };
-    if (force == 4) return go(w8a8_direct<4, TY>, 4);
-    if (force == 8) return go(w8a8_direct<8, TY>, 8);
-    return K > 2048 ? go(w8a8_direct<8, TY>, 8) : go(w8a8_direct<4, TY>, 4);
+    auto staged = [&](auto kernel, int TM, int TN) {
+        const int64_t tm = (T + TM - 1) / TM, tn = (NT + 4 * TN - 1) / (4 * TN);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(256), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
+                           (int)N, (int)U, (int)tm, (int)tn);
+        return launch_status();
+    };
+    switch (path_of(T, NT, K)) {
+        case kDirect: return direct(w8a8_direct<8, 1, 1, 4, TY>, 1, 1);
+        case kDirectLong: return direct(w8a8_direct<8, 2, 2, 2, TY>, 2, 2);
+        case kStaged64x128: return staged(w8a8_staged<2, 1, 4, 4, 2, TY>, 2, 1);
+        case kStaged64x256: return staged(w8a8_staged<2, 2, 4, 4, 2, TY>, 2, 2);
+        default: return staged(w8a8_staged<4, 2, 3, 3, 2, TY>, 4, 2);
+    }
 }
 
 bool known_dtype(int d) { return d == TIQ_F32 || d == TIQ_BF16; }
