@@ -173,58 +173,64 @@ __device__ __forceinline__ float finish(int sum, float sx, float sw, float b) {
     return fmaf((float)sum * sx, sw, b);
 }
 
-// The row's scale and codes in LDS for a product of few rows (M <= kFusedRows): W wavefronts,
-// W / Mp of them a row (Mp: M's next power of two), K <= kFusedK columns, the padding
-// columns zero. Row m's codes lie at m * 32 U.
-constexpr int kFusedRows = 4, kFusedK = 8192;
+// Scales and codes in LDS of a product's rows (few of them: rows_fused): the W wavefronts
+// share a row where there are more of them than rows, else take rows in turn. Row m's
+// codes lie at m * end, zero from K on.
+constexpr int kSmallRows = 16, kFusedBytes = 32768;
 template <int W, typename TX>
 __device__ __forceinline__ void quantize_rows(const TX* __restrict__ x, int64_t ldx, int M, int K, int end,
                                               int8_t* __restrict__ codes, float* __restrict__ scale,
                                               uint32_t* __restrict__ red) {
     constexpr int VEC = 16 / (int)sizeof(TX);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int Mp = M <= 1 ? 1 : M <= 2 ? 2 : 4, per = W / Mp;  // wavefronts a row
-    const int row = wave / per, c0 = ((wave - row * per) * 64 + lane) * VEC, step = per * 64 * VEC;
-    const TX* xr = x + (int64_t)min(row, M - 1) * ldx;
-    // `f` over the row's 16-byte pieces, past its end zeros
-    auto pieces = [&](auto f) {
-        for (int c = c0; c < end; c += 4 * step) {
-            float v[4][VEC];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int per = M <= 1 ? W : M <= 2 ? W / 2 : M <= 4 ? W / 4 : M <= 8 ? W / 8 : max(1, W / 16);  // wavefronts a row
+    const int c0 = ((wave % per) * 64 + lane) * VEC, step = per * 64 * VEC;
+    for (int row = wave / per; row < kSmallRows; row += W / per) {
+        if (row - wave / per >= M) break;  // (alike in every wavefront: no row left for any)
+        const TX* xr = x + (int64_t)min(row, M - 1) * ldx;
+        // `f` over the row's 16-byte pieces, past its end zeros
+        auto pieces = [&](auto f) {
+            for (int c = c0; c < end; c += 4 * step) {
+                float v[4][VEC];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_16(xr + min(c + step * i, K - VEC), v[i]);
+                for (int i = 0; i < 4; ++i) load_16(xr + min(c + step * i, K - VEC), v[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int ci = c + step * i;
-                if (ci >= end) break;
-                if (ci > K - VEC) {
+                for (int i = 0; i < 4; ++i) {
+                    const int ci = c + step * i;
+                    if (ci >= end) break;
+                    if (ci > K - VEC) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) v[i][e] = ci + e < K ? load_x(xr + ci + e) : 0.f;
+                        for (int e = 0; e < VEC; ++e) v[i][e] = ci + e < K ? load_x(xr + ci + e) : 0.f;
+                    }
+                    f(ci, v[i]);
                 }
-                f(ci, v[i]);
             }
-        }
-    };
-    uint32_t m = 0;
-    pieces([&](int, const float(&v)[VEC]) {
+        };
+        uint32_t m = 0;
+        pieces([&](int, const float(&v)[VEC]) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) m = umax(m, abs_bits(v[e]));
-    });
-    m = wave_max_u32(m);
-    if (lane == 0) red[wave] = m;
-    __syncthreads();
-    for (int w = 0; w < per; ++w) m = umax(m, red[row * per + w]);
-    const float s = scale_from_amax(__uint_as_float(m), 127.f), inv = 1.0f / s;
-    if (wave == row * per && lane == 0) scale[row] = s;
-    pieces([&](int c, const float(&v)[VEC]) {
-#pragma unroll
-        for (int g = 0; g < VEC / 4; ++g) {
-            int k[4];
-            codes4(make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]), s, inv, -128, 127, k);
-            *reinterpret_cast<uint32_t*>(codes + row * end + c + 4 * g) =
-                (uint32_t)(k[0] & 0xff) | (uint32_t)(k[1] & 0xff) << 8 | (uint32_t)(k[2] & 0xff) << 16 |
-                (uint32_t)(k[3] & 0xff) << 24;
+            for (int e = 0; e < VEC; ++e) m = umax(m, abs_bits(v[e]));
+        });
+        m = wave_max_u32(m);
+        if (per > 1) {  // then one turn is all
+            if (lane == 0) red[wave] = m;
+            __syncthreads();
+            for (int w = 0; w < per; ++w) m = umax(m, red[wave / per * per + w]);
         }
-    });
+        if (row >= M) continue;
+        const float s = scale_from_amax(__uint_as_float(m), 127.f), inv = 1.0f / s;
+        if (c0 == 0) scale[row] = s;
+        pieces([&](int c, const float(&v)[VEC]) {
+#pragma unroll
+            for (int g = 0; g < VEC / 4; ++g) {
+                int k[4];
+                codes4(make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]), s, inv, -128, 127, k);
+                *reinterpret_cast<uint32_t*>(codes + row * end + c + 4 * g) =
+                    (uint32_t)(k[0] & 0xff) | (uint32_t)(k[1] & 0xff) << 8 | (uint32_t)(k[2] & 0xff) << 16 |
+                    (uint32_t)(k[3] & 0xff) << 24;
+            }
+        });
+    }
 }
 
 // The product of up to 16 rows: a workgroup of W wavefronts per 16 output columns, the K
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(64 * W) void w8a8_small(const TX* __restrict__ x, i
                                                      int M, int N, int K, int U) {
     constexpr int PF = 4;
     __shared__ int part[W][256];
-    __shared__ float scale[FUSE ? kFusedRows : 1];
+    __shared__ float scale[FUSE ? kSmallRows : 1];
     __shared__ uint32_t red[W];
     extern __shared__ __attribute__((aligned(16))) int8_t codes[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -608,6 +614,16 @@ int launch_tokens(const TX* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, 
 //     20.2 against 24.9 with 64 x 256; 8192 x 768 x 2304: 37.5 against 33.5);
 //   64 x 256 where those are many (2048 x 1600 x 1600, 224 of them: 17.4 against 18.7 with
 //     64 x 128; 1024 x 1600 x 1600, 112: 13.6 against 12.4), else 64 x 128.
+// Whether the product quantizes its rows itself (then it takes no workspace): up to 8
+// rows, up to 16 where they are short. (us in a graph, so / by a launch of their own before,
+// which an eager call's host also waits 4 us for: 1 x 768 x 2304 3.6 / 5.3, 8 x 768 x 2304
+// 4.3 / 5.3, 4 x 6400 x 1600 7.7 / 9.1, 8 x 4096 x 1024 7.5 / 6.9, 16 x 768 x 2304 5.9 / 5.3,
+// 16 x 1600 x 6400 10.7 / 6.6.)
+bool rows_fused(int x_dtype, int64_t M, int64_t K) {
+    const int64_t bytes = M * 32 * units_of(K);  // of codes, in LDS
+    return M <= kSmallRows && bytes <= (M <= 8 ? kFusedBytes : 12544) && K >= (x_dtype == TIQ_F32 ? 4 : 8);
+}
+
 enum Path { kDirect, kDirectLong, kStaged64x128, kStaged64x256, kStaged128x256 };
 
 Path path_of(int64_t T, int64_t NT, int64_t K) {
@@ -629,15 +645,13 @@ int run_w8a8(const TX* x, int64_t M, int64_t K, int64_t ldx, const int8_t* wt, c
                            y, ldy, (int)M, (int)N, (int)K, (int)U);
         return launch_status();
     };
-    // (us in a graph, rows quantized by the workgroups / by a launch before: 1 x 768 x 2304
-    // 3.5 / 5.3, 1 x 6400 x 1600 5.4 / 9.2, 4 x 6400 x 1600 8.0 / 9.1)
-    if (M <= kFusedRows && K <= kFusedK && K >= 16 / (int)sizeof(TX)) {
+    if (rows_fused(sizeof(TX) == 4 ? TIQ_F32 : TIQ_BF16, M, K)) {
         const size_t lds = (size_t)(M * 32 * U);
         return K > 2048 ? small(w8a8_small<16, true, TX, TY>, 16, lds) : small(w8a8_small<8, true, TX, TY>, 8, lds);
     }
     const int rc = launch_tokens<true>(x, M, K, ldx, xt, (int64_t)0, sx, st);
     if (rc != TIQ_OK) return rc;
-    if (M <= 16) return K > 2048 ? small(w8a8_small<16, false, TX, TY>, 16, 0) : small(w8a8_small<8, false, TX, TY>, 8, 0);
+    if (M <= kSmallRows) return K > 2048 ? small(w8a8_small<16, false, TX, TY>, 16, 0) : small(w8a8_small<8, false, TX, TY>, 8, 0);
     auto direct = [&](auto kernel, int TM, int TN) {
         const int64_t tm = (T + TM - 1) / TM, tn = (NT + TN - 1) / TN;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(512), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
@@ -704,8 +718,8 @@ extern "C" int tiq_w8a8_untile(const int8_t* tiles, int64_t N, int64_t K, int8_t
     return launch_status();
 }
 
-extern "C" size_t tiq_linear_w8a8_workspace(int64_t M, int64_t K, int64_t N) {
-    if (M <= 0 || K <= 0 || N <= 0) return 0;
+extern "C" size_t tiq_linear_w8a8_workspace(int x_dtype, int64_t M, int64_t K, int64_t N) {
+    if (!known_dtype(x_dtype) || M <= 0 || K <= 0 || N <= 0 || rows_fused(x_dtype, M, K)) return 0;
     return round256((size_t)(tiles_of(M) * (units_of(K) * 1024 + 128)));  // (scales of whole tiles)
 }
 
@@ -720,8 +734,8 @@ extern "C" int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K,
         return TIQ_EALIGN;
     if (K > kMaxK || M > 0x7fffffc0LL || N > 0x7fffffc0LL || tiles_of(M) * tiles_of(N) > 0x7fffffffLL)
         return TIQ_EUNSUPPORTED;
-    if (!workspace || workspace_bytes < tiq_linear_w8a8_workspace(M, K, N) || !aligned(workspace, 16))
-        return TIQ_EWORKSPACE;
+    const size_t need = tiq_linear_w8a8_workspace(x_dtype, M, K, N);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return TIQ_EWORKSPACE;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     hipStream_t st = as_stream(stream);
     if (x_dtype == TIQ_F32) {

@@ -239,12 +239,13 @@ def _w8a8_into(m: QuantLinear, x2: torch.Tensor, y: torch.Tensor) -> None:
             return _w8a8_into(m, x2, y)
     L = _lib.lib()
     M, K = x2.shape
-    N = m.out_features
-    ws_bytes = L.tiq_linear_w8a8_workspace(M, K, N)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x2.device)
-    rc = L.tiq_linear_w8a8(x2.data_ptr(), _lib.dtype_code(x2.dtype), M, K, x2.stride(0), codes.data_ptr(),
-                           scale.data_ptr(), None if bias is None else bias.data_ptr(), N, y.data_ptr(),
-                           _lib.dtype_code(y.dtype), y.stride(0), ws.data_ptr(), ws_bytes, _lib.stream_of(x2))
+    N, xd = m.out_features, _lib.dtype_code(x2.dtype)
+    ws_bytes = L.tiq_linear_w8a8_workspace(xd, M, K, N)
+    ws = x2.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    rc = L.tiq_linear_w8a8(x2.data_ptr(), xd, M, K, x2.stride(0), codes.data_ptr(), scale.data_ptr(),
+                           None if bias is None else bias.data_ptr(), N, y.data_ptr(),
+                           xd if y.dtype is x2.dtype else _lib.dtype_code(y.dtype), y.stride(0),
+                           None if ws is None else ws.data_ptr(), ws_bytes, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, f"quantized linear (w8a8, M={M}, K={K}, N={N})")
 

@@ -96,7 +96,7 @@ class _TokenLogprobs(torch.autograd.Function):
     def forward(ctx, logits, tokens, top, ignore_index):
         logprob, entropy, stats, ids, values = _forward(logits, tokens, top, ignore_index, True)
         ctx.set_materialize_grads(False)
-        ctx.stats, ctx.top, ctx.ignore_index = stats, top, ignore_index
+        ctx.stats, ctx.options = stats, (top, ignore_index)
         if top:
             ctx.mark_non_differentiable(ids)
             ctx.save_for_backward(logits, tokens, entropy, ids)
@@ -111,13 +111,14 @@ class _TokenLogprobs(torch.autograd.Function):
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None, None
         logits, tokens, entropy, *ids = ctx.saved_tensors
+        top, ignore_index = ctx.options
         gl, gh, gt = _as_weight(g_logprob), _as_weight(g_entropy), _as_weight(g_top)
         x, batch, rows, sb, sr = _rows_of(logits)
         grad = logits.new_empty(logits.shape)
         rc = _lib.lib().tiq_token_logprobs_grad(
             x.data_ptr(), _lib.F32 if x.dtype is torch.float32 else _lib.BF16, batch, rows, sb, sr, x.shape[-1],
-            tokens.data_ptr(), ctx.ignore_index, ctx.stats.data_ptr(), entropy.data_ptr(),
-            None if gl is None else gl.data_ptr(), None if gh is None else gh.data_ptr(), ctx.top,
+            tokens.data_ptr(), ignore_index, ctx.stats.data_ptr(), entropy.data_ptr(),
+            None if gl is None else gl.data_ptr(), None if gh is None else gh.data_ptr(), top,
             ids[0].data_ptr() if ids else None, None if gt is None else gt.data_ptr(), grad.data_ptr(),
             _lib.stream_of(x))
         if rc:

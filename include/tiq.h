@@ -629,8 +629,9 @@ int tiq_w8a8_untile(const int8_t* tiles, int64_t N, int64_t K, int8_t* q, void* 
  * more where y is bf16. No counterpart in the reference: it takes the place of
  * F.linear on W_hat (model.py:254,319,352,355) where activations may be coded too.
  * x (M, K) and y (M, N) fp32 or bf16, at any alignment of their elements. The
- * workspace is 16-byte aligned. */
-size_t tiq_linear_w8a8_workspace(int64_t M, int64_t K, int64_t N);
+ * workspace holds the rows' tiles and scales, 16-byte aligned (0 bytes, and NULL, for
+ * few rows, which the product quantizes itself). */
+size_t tiq_linear_w8a8_workspace(int x_dtype, int64_t M, int64_t K, int64_t N);
 int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const int8_t* w_tiles,
                     const float* scale, const float* bias, int64_t N, void* y, int y_dtype, int64_t ldy,
                     void* workspace, size_t workspace_bytes, void* stream);

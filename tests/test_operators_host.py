@@ -43,9 +43,15 @@ def test_tiles_arguments():
 def test_linear_w8a8_arguments():
     L = _lib.load()
     f = L.tiq_linear_w8a8
-    need = L.tiq_linear_w8a8_workspace(3, 64, 5)
-    assert need >= 3 * 64 + 3 * 4 and L.tiq_linear_w8a8_workspace(0, 64, 5) == 0
-    ok = dict(x=16, xd=0, M=3, K=64, ldx=64, w=16, s=16, b=None, N=5, y=16, yd=0, ldy=5, ws=16, nb=need)
+    need = L.tiq_linear_w8a8_workspace(0, 17, 64, 5)
+    assert need >= 32 * 64 + 32 * 4 and L.tiq_linear_w8a8_workspace(0, 0, 64, 5) == 0
+    assert L.tiq_linear_w8a8_workspace(2, 17, 64, 5) == 0
+    # few rows the product quantizes itself: of 16 bytes at least, 32 KB of codes at most
+    assert L.tiq_linear_w8a8_workspace(0, 8, 4096, 5) == 0 and L.tiq_linear_w8a8_workspace(0, 8, 4097, 5) > 0
+    assert L.tiq_linear_w8a8_workspace(0, 16, 768, 5) == 0 and L.tiq_linear_w8a8_workspace(0, 16, 1600, 5) > 0
+    assert L.tiq_linear_w8a8_workspace(0, 4, 64, 5) == 0 and L.tiq_linear_w8a8_workspace(0, 4, 3, 5) > 0
+    assert L.tiq_linear_w8a8_workspace(1, 4, 8, 5) == 0 and L.tiq_linear_w8a8_workspace(1, 4, 7, 5) > 0
+    ok = dict(x=16, xd=0, M=17, K=64, ldx=64, w=16, s=16, b=None, N=5, y=16, yd=0, ldy=5, ws=16, nb=need)
 
     def call(**kw):
         return f(*{**ok, **kw}.values(), None)

@@ -185,8 +185,8 @@ def test_strided_input_and_output_through_the_library(dev, m, k, n, dtype):
     lin = _linear(q, s, b, dev)
     out = torch.full((m + 2, n + 7), 5.0, dtype=dtype, device=dev)
     L = _lib.lib()
-    nb = L.tiq_linear_w8a8_workspace(m, k, n)
-    ws = torch.full((nb,), 0x7F, dtype=torch.uint8, device=dev)
+    nb = L.tiq_linear_w8a8_workspace(_lib.dtype_code(dtype), m, k, n)
+    ws = torch.full((max(nb, 1),), 0x7F, dtype=torch.uint8, device=dev)
     rc = L.tiq_linear_w8a8(x.data_ptr(), _lib.dtype_code(dtype), m, k, x.stride(0), lin.codes.data_ptr(),
                            lin.scale.data_ptr(), lin.bias.data_ptr(), n, out[:, 3:].data_ptr(),
                            _lib.dtype_code(dtype), n + 7, ws.data_ptr(), nb, _lib.stream_of(x))
