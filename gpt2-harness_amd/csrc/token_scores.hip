@@ -158,7 +158,7 @@ __device__ __forceinline__ void hold(uint64_t* keys, int* count, float xj, int j
     if (c < kCap) keys[c] = place_key(xj, j);
 }
 
-// The top-th largest of 64 numbers in LDS, in every lane.
+// The top-th largest of 64 numbers in LDS, in every lane (any of them where one is NaN).
 __device__ __forceinline__ float kth_of_64(const float* q, int top) {
     const int lane = threadIdx.x & 63;
     const float mine = q[lane];
@@ -170,7 +170,7 @@ __device__ __forceinline__ float kth_of_64(const float* q, int top) {
                 (v.z > mine || (v.z == mine && i + 2 < lane)) + (v.w > mine || (v.w == mine && i + 3 < lane));
     }
     const uint64_t kth = __ballot(rank == top - 1);
-    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), __builtin_ctzll(kth)));
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), kth ? __builtin_ctzll(kth) : 0));
 }
 
 // With every logit above `bound` of places first .. last - 1 held: of those equal to it
@@ -269,8 +269,8 @@ struct Row {
 // the row's maximum, for d. ONE: a batch a thread is the whole of it, and the logits
 // are looked at again in the registers.
 template <typename TX, int T, int B, bool ONE>
-__global__ __launch_bounds__(T) void scores_kernel(const TX* __restrict__ x, int64_t rows, int64_t sb, int64_t sr,
-                                                   int V, int S, int per, Scores o, Part* __restrict__ parts,
+__global__ __launch_bounds__(T) void scores_kernel(const TX* __restrict__ x, int64_t row0, int64_t rows, int64_t sb,
+                                                   int64_t sr, int V, int S, int per, Scores o, Part* __restrict__ parts,
                                                    uint64_t* __restrict__ part_keys) {
     constexpr int VEC = kVec<TX>, W = T / 64;
     __shared__ __attribute__((aligned(16))) uint64_t keys[kCap + 8];
@@ -278,8 +278,9 @@ __global__ __launch_bounds__(T) void scores_kernel(const TX* __restrict__ x, int
     __shared__ float wmax[W], wsum[W], wsum1[W], result[2];
     __shared__ int wowner[W], owners[ONE ? 1 : T], listed[1], count[1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x / (unsigned)S;
-    const int seg = (int)(blockIdx.x - row * S);
+    const unsigned r0 = blockIdx.x / (unsigned)S;
+    const int64_t row = row0 + r0;
+    const int seg = (int)(blockIdx.x - r0 * S);
     const Row<TX> r(row_at(x, row, rows, sb, sr), V);
     const int v0 = seg * per, v1 = min(r.nvec, v0 + per);
     auto extra_of = [&](int t) { return r.extra(t, seg == 0, seg == S - 1); };
@@ -597,13 +598,13 @@ __device__ __forceinline__ u32x4 packed(const float (&v)[8]) {
 // scores' pass and this one, again and again: 105 + 141 us; from the last row 98 + 136;
 // past the cache too 69 + 136.
 template <typename TX, bool PAST>
-__global__ __launch_bounds__(kThreads) void grad_kernel(const TX* __restrict__ x, int64_t rows, int64_t sb, int64_t sr,
-                                                        int V, int chunks, int per, Grads o, TX* grad) {
+__global__ __launch_bounds__(kThreads) void grad_kernel(const TX* __restrict__ x, int64_t row0, int64_t rows, int64_t sb,
+                                                        int64_t sr, int V, int chunks, int per, Grads o, TX* grad) {
     constexpr int VEC = kVec<TX>;
     const int tid = threadIdx.x;
     const unsigned id = gridDim.x - 1 - blockIdx.x;  // the last rows first
-    const int64_t row = id / (unsigned)chunks;
-    const int chunk = (int)(id - row * chunks);
+    const int64_t row = row0 + id / (unsigned)chunks;
+    const int chunk = (int)(id % (unsigned)chunks);
     const TX* xr = row_at(x, row, rows, sb, sr);
     TX* gr = grad + row * V;
     const int head = min(V, (int)((16 - ((uintptr_t)gr & 15)) & 15) / (int)sizeof(TX));
@@ -688,23 +689,27 @@ int check_rows(const void* logits, int dtype, int64_t batch, int64_t rows, int64
 
 using namespace tiq;
 
+// Rows a launch: its threads are counted in 32 bits.
+constexpr int64_t kLaunchRows = 1 << 22;
+
 template <typename TX>
 static int run_scores(const TX* x, int64_t count, int64_t rows, int64_t sb, int64_t sr, int V, const Plan& p,
                       const Scores& o, void* workspace, hipStream_t st) {
     Part* parts = static_cast<Part*>(workspace);
     uint64_t* keys = reinterpret_cast<uint64_t*>(parts + (p.S > 1 ? count * p.S : 0));
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(count * p.S)), dim3(p.T), 0, st, x, rows, sb, sr, V, p.S, p.per, o,
-                           parts, keys);
-    };
-    switch (p.T * 100 + p.B * 10 + p.one) {
-        case 6411: go(scores_kernel<TX, 64, 1, true>); break;
-        case 6421: go(scores_kernel<TX, 64, 2, true>); break;
-        case 6441: go(scores_kernel<TX, 64, 4, true>); break;
-        case 25641: go(scores_kernel<TX, 256, 4, true>); break;
-        case 25640: go(scores_kernel<TX, 256, 4, false>); break;
-        case 51240: go(scores_kernel<TX, 512, 4, false>); break;
-        default: return TIQ_EUNSUPPORTED;
+    for (int64_t r0 = 0; r0 < count; r0 += kLaunchRows) {  // (cut rows are few: one launch)
+        const unsigned groups = (unsigned)(std::min(count - r0, kLaunchRows) * p.S);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(groups), dim3(p.T), 0, st, x, r0, rows, sb, sr, V, p.S, p.per, o, parts, keys);
+        };
+        if (p.T == 512) go(scores_kernel<TX, 512, 4, false>);
+        else if (p.T == 256 && p.one) go(scores_kernel<TX, 256, 4, true>);
+        else if (p.T == 256) go(scores_kernel<TX, 256, 4, false>);
+        else if (p.B == 1) go(scores_kernel<TX, 64, 1, true>);
+        else if (p.B == 2) go(scores_kernel<TX, 64, 2, true>);
+        else go(scores_kernel<TX, 64, 4, true>);
+        const int rc = launch_status();
+        if (rc != TIQ_OK) return rc;
     }
     if (p.S > 1)
         hipLaunchKernelGGL(join_kernel<TX>, dim3((unsigned)count), dim3(kThreads), 0, st, x, rows, sb, sr, V, p.S, o,
@@ -737,19 +742,24 @@ extern "C" int tiq_token_logprobs(const void* logits, int dtype, int64_t batch, 
                       workspace, as_stream(stream));
 }
 
-// Four vectors a thread.
+// Four vectors a thread. The launches go from the last rows to the first, as each of them does.
 template <typename TX>
 static int run_grad(const TX* x, int64_t count, int64_t rows, int64_t sb, int64_t sr, int V, const Grads& o, TX* grad,
                     hipStream_t st) {
     const int64_t vectors = std::max(1, V / kVec<TX>);
     int per = 4 * kThreads;
     int64_t chunks = (vectors + per - 1) / per;
-    if (chunks * count > 0x7fffffffLL) per = (int)vectors, chunks = 1;
+    const int64_t part = std::max<int64_t>(1, std::min(kLaunchRows, kLaunchRows / chunks));
     // logits and gradient together beyond the cache's 256 MB
     const bool past = count * V * (int64_t)sizeof(TX) > (128 << 20);
-    hipLaunchKernelGGL((past ? grad_kernel<TX, true> : grad_kernel<TX, false>), dim3((unsigned)(count * chunks)),
-                       dim3(kThreads), 0, st, x, rows, sb, sr, V, (int)chunks, per, o, grad);
-    return launch_status();
+    for (int64_t r0 = (count - 1) / part * part; r0 >= 0; r0 -= part) {
+        const int64_t n = std::min(count - r0, part);
+        hipLaunchKernelGGL((past ? grad_kernel<TX, true> : grad_kernel<TX, false>), dim3((unsigned)(n * chunks)),
+                           dim3(kThreads), 0, st, x, r0, rows, sb, sr, V, (int)chunks, per, o, grad);
+        const int rc = launch_status();
+        if (rc != TIQ_OK) return rc;
+    }
+    return TIQ_OK;
 }
 
 extern "C" int tiq_token_logprobs_grad(const void* logits, int dtype, int64_t batch, int64_t rows,

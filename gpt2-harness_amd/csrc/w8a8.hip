@@ -142,28 +142,28 @@ __global__ __launch_bounds__(TH) void tokens_kernel(const TX* __restrict__ x, in
     }
 }
 
-// Weight codes (N, K) -> tiles, a thread per 16 bytes of them.
+// Weight codes (N, K) -> tiles, 16 bytes of them a thread at a time.
 __global__ __launch_bounds__(256) void tile_weight_kernel(const int8_t* __restrict__ w, int64_t N, int64_t K,
                                                           int64_t ldw, int64_t U, int64_t chunks,
                                                           int8_t* __restrict__ tiles) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= chunks) return;
-    const int64_t b = i >> 6, t = b / U, u = b - t * U;
-    const int l = (int)(i & 63);
-    const int64_t n = 32 * t + (l & 31), k = 32 * u + 16 * (l >> 5);
-    int8_t c[16];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+        const int64_t b = i >> 6, t = b / U, u = b - t * U;
+        const int l = (int)(i & 63);
+        const int64_t n = 32 * t + (l & 31), k = 32 * u + 16 * (l >> 5);
+        int8_t c[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) c[j] = n < N && k + j < K ? w[n * ldw + k + j] : (int8_t)0;
-    int4 v;
-    __builtin_memcpy(&v, c, 16);
-    *reinterpret_cast<int4*>(tiles + i * 16) = v;
+        for (int j = 0; j < 16; ++j) c[j] = n < N && k + j < K ? w[n * ldw + k + j] : (int8_t)0;
+        int4 v;
+        __builtin_memcpy(&v, c, 16);
+        *reinterpret_cast<int4*>(tiles + i * 16) = v;
+    }
 }
 
-// Tiles -> codes (N, K), a thread per code.
+// Tiles -> codes (N, K), a code a thread at a time.
 __global__ __launch_bounds__(256) void untile_weight_kernel(const int8_t* __restrict__ tiles, int64_t K, int64_t U,
                                                             int64_t count, int8_t* __restrict__ w) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) w[i] = tiles[tile_byte(i / K, i % K, U)];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256)
+        w[i] = tiles[tile_byte(i / K, i % K, U)];
 }
 
 __device__ __forceinline__ void store_y(float* p, float v) { *p = v; }
@@ -581,27 +581,41 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
             }
 }
 
+// Workgroups of 256 for n pieces of work; each goes on to further ones past 2^20 of them.
+unsigned groups_of(int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20); }
+
 size_t round256(size_t b) { return (b + 255) / 256 * 256; }
+
+// Rows a launch: its threads are counted in 32 bits.
+constexpr int64_t kTokenRows = 1 << 22;
 
 template <bool TILES, typename TX>
 int launch_tokens(const TX* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                   hipStream_t st) {
     constexpr int VEC = 16 / (int)sizeof(TX);
-    auto held = [&](auto kernel, int threads) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + 3) / 4)), dim3(threads), 0, st, x, ldx, (int)rows, (int)K,
-                           q, ldq, units_of(K), scale);
-        return launch_status();
-    };
-    // passes over the columns a row has, with its padding
-    const int64_t cols = TILES ? 32 * units_of(K) : K, small = (cols + 64 * VEC - 1) / (64 * VEC);
-    if (K >= VEC && small <= 2) return held(tokens_kernel<TILES, 2, 256, TX>, 256);
-    if (K >= VEC && small <= 4) return held(tokens_kernel<TILES, 4, 256, TX>, 256);
-    if (K >= VEC && small <= 8) return held(tokens_kernel<TILES, 8, 256, TX>, 256);
-    if (K >= VEC && small <= 16) return held(tokens_kernel<TILES, 4, 1024, TX>, 1024);
-    if (K >= VEC && small <= 32) return held(tokens_kernel<TILES, 8, 1024, TX>, 1024);
-    hipLaunchKernelGGL((tokens_generic<TILES, TX>), dim3((unsigned)rows), dim3(256), 0, st, x, ldx, K, q, ldq,
-                       units_of(K), scale);
-    return launch_status();
+    const int64_t U = units_of(K);
+    // passes of 256 threads over the columns a row has, with its padding
+    const int64_t cols = TILES ? 32 * U : K, passes = (cols + 64 * VEC - 1) / (64 * VEC);
+    for (int64_t r0 = 0; r0 < rows; r0 += kTokenRows) {
+        const int n = (int)std::min(rows - r0, kTokenRows);
+        const TX* xr = x + r0 * ldx;
+        int8_t* qr = q + (TILES ? r0 / 32 * U * 1024 : r0 * ldq);
+        auto held = [&](auto kernel, int threads) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((n + 3) / 4)), dim3(threads), 0, st, xr, ldx, n, (int)K, qr, ldq, U,
+                               scale + r0);
+        };
+        if (K < VEC || passes > 32)
+            hipLaunchKernelGGL((tokens_generic<TILES, TX>), dim3((unsigned)n), dim3(256), 0, st, xr, ldx, K, qr, ldq, U,
+                               scale + r0);
+        else if (passes <= 2) held(tokens_kernel<TILES, 2, 256, TX>, 256);
+        else if (passes <= 4) held(tokens_kernel<TILES, 4, 256, TX>, 256);
+        else if (passes <= 8) held(tokens_kernel<TILES, 8, 256, TX>, 256);
+        else if (passes <= 16) held(tokens_kernel<TILES, 4, 1024, TX>, 1024);
+        else held(tokens_kernel<TILES, 8, 1024, TX>, 1024);
+        const int rc = launch_status();
+        if (rc != TIQ_OK) return rc;
+    }
+    return TIQ_OK;
 }
 
 // How a product over more than 16 rows is taken, by its 32 x 32 output tiles (rows' T,
@@ -702,9 +716,8 @@ extern "C" int tiq_w8a8_tile(const int8_t* q, int64_t N, int64_t K, int64_t ldq,
     if (!q || !tiles || ldq < K) return TIQ_EINVAL;
     if (!aligned(tiles, 16)) return TIQ_EALIGN;
     const int64_t U = units_of(K), chunks = tiles_of(N) * U * 64;
-    if (chunks / 256 > 0x7fffffffLL) return TIQ_EUNSUPPORTED;
-    hipLaunchKernelGGL(tile_weight_kernel, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, as_stream(stream), q,
-                       N, K, ldq, U, chunks, tiles);
+    hipLaunchKernelGGL(tile_weight_kernel, dim3(groups_of(chunks)), dim3(256), 0, as_stream(stream), q, N, K, ldq, U,
+                       chunks, tiles);
     return launch_status();
 }
 
@@ -712,9 +725,8 @@ extern "C" int tiq_w8a8_untile(const int8_t* tiles, int64_t N, int64_t K, int8_t
     if (N < 0 || K < 0) return TIQ_EINVAL;
     if (N == 0 || K == 0) return TIQ_OK;
     if (!q || !tiles) return TIQ_EINVAL;
-    if ((N * K + 255) / 256 > 0x7fffffffLL) return TIQ_EUNSUPPORTED;
-    hipLaunchKernelGGL(untile_weight_kernel, dim3((unsigned)((N * K + 255) / 256)), dim3(256), 0, as_stream(stream),
-                       tiles, K, units_of(K), N * K, q);
+    hipLaunchKernelGGL(untile_weight_kernel, dim3(groups_of(N * K)), dim3(256), 0, as_stream(stream), tiles, K,
+                       units_of(K), N * K, q);
     return launch_status();
 }
 
@@ -732,8 +744,8 @@ extern "C" int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K,
     if (!aligned(x, x_dtype == TIQ_F32 ? 4 : 2) || !aligned(y, y_dtype == TIQ_F32 ? 4 : 2) || !aligned(w_tiles, 16) ||
         !aligned(scale, 4) || !aligned(bias, 4))
         return TIQ_EALIGN;
-    if (K > kMaxK || M > 0x7fffffc0LL || N > 0x7fffffc0LL || tiles_of(M) * tiles_of(N) > 0x7fffffffLL)
-        return TIQ_EUNSUPPORTED;
+    // (threads of a launch are counted in 32 bits)
+    if (K > kMaxK || M > 0x7fffffc0LL || N > 1 << 26 || tiles_of(M) * tiles_of(N) > 1 << 26) return TIQ_EUNSUPPORTED;
     const size_t need = tiq_linear_w8a8_workspace(x_dtype, M, K, N);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return TIQ_EWORKSPACE;
     uint8_t* ws = static_cast<uint8_t*>(workspace);

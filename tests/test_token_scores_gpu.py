@@ -527,3 +527,68 @@ def test_second_derivatives_are_refused(dev):
     s = g.token_logprobs(leaf, tokens.to(dev))
     with pytest.raises(RuntimeError, match="no second derivative"):
         torch.autograd.grad(s.logprob.sum(), leaf, create_graph=True)
+
+
+def _check_top_on_gpu(x, out, top):
+    """Alternatives of GPU logits against a stable sort in 64 bits."""
+    values, ids = (x.double() + 0.0).sort(dim=1, descending=True, stable=True)
+    assert torch.equal(out.top_ids, ids[:, :top])
+    want = torch.log_softmax(x.double(), dim=1).gather(1, ids[:, :top])
+    got = out.top_logprobs.double()
+    ok = bool(((got == want) | ((got - want).abs() <= 1e-5 * (1 + want.abs()))).all())
+    assert ok
+
+
+@pytest.mark.parametrize("rows,threads", [(1030, 512), (600, 256), (40, 256), (3, 256)])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_large_logits_in_few_places(dev, rows, threads, dtype):
+    """Rows whose large logits all fall to a few threads, ties by the thousand, rows with
+    fewer tokens left than alternatives wanted: every way the selection can go."""
+    v, vec = 20000, 16 // (4 if dtype is FP32 else 2)
+    gen = torch.Generator(device=dev).manual_seed(18)
+    x = torch.randn(rows, v, generator=gen, device=dev)
+    place = torch.arange(v, device=dev)
+    few = (place // vec) % threads < 8 * threads // 64
+    x[0::5] += 50.0 * few
+    x[1::5] = 1.5                                     # all equal
+    x[2::5, 20:] = float("-inf")                      # as many left as wanted, or fewer
+    x[2::10, 7:] = float("-inf")
+    x[3::5] = torch.where(place % 3 == 0, 2.0, x[3::5])  # thousands of ties below a few larger ones
+    x[3::5, 777] = 9.0
+    x = x.to(dtype)
+    for top in (4, 20, MAX_TOP):
+        _check_top_on_gpu(x, g.token_logprobs(x, torch.zeros(rows, dtype=torch.int64, device=dev), top=top), top)
+
+
+@pytest.mark.parametrize("rows,v", [(2, 40), (3, 1003), (2, 9001), (1030, 9001)])
+def test_signalling_nans(dev, rows, v):
+    """NaN bits of every kind give NaN scores and the top place, and touch no other row."""
+    for dtype, bits in ((FP32, (0x7F800001, -0x3FFFFF, 0x7FC00000)), (BF16, (0x7F81, -0x7F, 0x7FC0))):
+        x, tokens = _logits(min(rows, 8), v, 19, dtype)
+        x = x.repeat(-(-rows // len(x)), 1)[:rows].to(dev)
+        tokens = tokens.repeat(-(-rows // len(tokens)))[:rows].to(dev)
+        clean = g.token_logprobs(x, tokens, top=3)
+        for b in bits:
+            y = x.clone()
+            y.view(torch.int32 if dtype is FP32 else torch.int16)[0, v - 2] = b
+            out = g.token_logprobs(y, tokens, top=3)
+            assert torch.isnan(out.logprob[0]) and torch.isnan(out.entropy[0]) and torch.isnan(out.top_logprobs[0]).all()
+            assert out.top_ids[0, 0] == v - 2
+            for a, c in zip(out, clean):
+                assert torch.equal(a[1:], c[1:])
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_more_rows_than_one_launch_takes(dev, dtype):
+    rows, v = (1 << 22) + 37, 9
+    gen = torch.Generator(device=dev).manual_seed(20)
+    x = torch.randn(rows, v, generator=gen, device=dev).to(dtype).requires_grad_()
+    tokens = torch.randint(0, v, (rows,), generator=gen, device=dev)
+    s = g.token_logprobs(x, tokens, top=2)
+    logp = torch.log_softmax(x.detach().double(), dim=1)
+    assert (s.logprob - logp.gather(1, tokens[:, None])[:, 0]).abs().max() < 2e-6
+    assert (s.entropy + (logp.exp() * logp).sum(dim=1)).abs().max() < 2e-6
+    assert torch.equal(s.top_ids[:, 0], x.detach().float().argmax(dim=1)) or dtype is BF16
+    (grad,) = torch.autograd.grad(s.logprob.sum(), x)
+    want = F.one_hot(tokens, v) - logp.exp()
+    assert (grad.double() - want).abs().max() < (2e-6 if dtype is FP32 else 2.0**-8)

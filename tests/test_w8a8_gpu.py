@@ -354,3 +354,22 @@ def test_refusals(dev):
         _linear(q, s, b, dev)(torch.zeros(2, 15, device=dev))
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         _linear(q, s, b, dev)(torch.zeros(2, 16))
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_more_rows_than_one_launch_takes(dev, dtype):
+    m, k, n = (1 << 22) + 37, 12, 3
+    gen = torch.Generator(device=dev).manual_seed(21)
+    x = torch.randn(m, k, generator=gen, device=dev).to(dtype)
+    qx, sx = g.quantize_tokens(x)
+    q2, s2 = g.quantize_tensor(x.float(), 8)
+    assert torch.equal(qx, q2) and torch.equal(sx, s2)
+    q, s, b = _weight(n, k, 22)
+    y = _linear(q, s, b, dev)(x).double()
+    core = (qx.double() @ q.to(dev).double().t()) * sx.double() * s.to(dev).double()
+    want = core + b.to(dev).double()
+    bound = core.abs() * 2.0**-22 + want.abs() * 2.0**-23
+    if dtype is BF16:
+        bound = bound + (want.abs() + bound) * 2.0**-8
+    ok = bool(((y - want).abs() <= bound).all())
+    assert ok
