@@ -541,11 +541,13 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const TX* __restrict__ x
 
 // How rows of n vectors are taken. Up to 256 vectors, a wavefront a row; up to 1024, a
 // workgroup of 256 with a batch a thread (5000 rows of 1003 bf16: 8.6 us against 15 with
-// 256 threads a row). Longer rows are cut into segments until there are about 1024
-// workgroups, each of a batch a thread at least, and no more segments than make the
-// join's keys many (64 rows of 131071 bf16 with 20 alternatives, in 8 / 16 segments: the
-// segments 10.7 / 11.5 us, the join 3.9 / 7.5). Uncut rows: 512 threads (4096 rows of
-// 50257 fp32, 256 / 512 / 1024 threads: 152 / 143 / 141 us; bf16 112 / 103 / 109).
+// 256 threads a row); longer ones, 512 threads (4096 rows of 50257 fp32, 256 / 512 / 1024
+// threads: 152 / 143 / 141 us; bf16 112 / 103 / 109). Only few and long rows are cut into
+// segments, which a second launch joins: about 1024 workgroups, no more segments than keep
+// the join's keys few (64 rows of 131071 with 20 alternatives, in 8 / 16: the join 3.9 /
+// 7.5 us). Whole / cut, in a graph with 5 alternatives: one row of 50257 fp32 9.4 / 9.3 (an
+// eager call 13.7 / 18.3, for the host's second launch), 131071 13.8 / 10.0, 262147 21.6 /
+// 11.0; 256 rows of 131071 29.1 / 36.5.
 struct Plan {
     int T, B;  // threads, vectors a batch
     bool one;  // a batch a thread
@@ -555,10 +557,10 @@ Plan plan_of(int dtype, int64_t rows, int64_t vocab, int top) {
     const int64_t n = std::max<int64_t>(1, vocab / (dtype == TIQ_F32 ? 4 : 8));
     if (n <= 256) return {64, n <= 64 ? 1 : n <= 128 ? 2 : 4, true, 1, (int)n};
     if (n <= 1024) return {256, 4, true, 1, (int)n};
+    if (n <= 16384 || rows >= 128) return {512, 4, false, 1, (int)n};
     int64_t S = std::min((n + 1023) / 1024, (1024 + rows - 1) / rows);
-    S = std::max<int64_t>(1, std::min<int64_t>(S, top ? std::max(4, 160 / top) : kThreads));
+    S = std::min<int64_t>(S, top ? std::max(4, 160 / top) : kThreads);
     const int per = (int)((n + S - 1) / S);
-    if (S == 1) return {512, 4, false, 1, per};
     return {256, 4, per <= 1024, (int)S, per};
 }
 

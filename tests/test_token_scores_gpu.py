@@ -105,7 +105,7 @@ def test_scores_against_64_bits(dev, rows, v, dtype, top):
     _check(g.token_logprobs(x.to(dev), tokens.to(dev), top=top), x, tokens, top)
 
 
-@pytest.mark.parametrize("rows,v", [(3, 50257), (600, 1003), (5, 131072)])
+@pytest.mark.parametrize("rows,v", [(3, 50257), (600, 1003), (5, 131072), (2, 262147)])
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 def test_sure_rows_keep_their_digits(dev, rows, v, dtype):
     """log p of a token that the model is sure of, far below 2^-24, to full precision."""
@@ -117,7 +117,7 @@ def test_sure_rows_keep_their_digits(dev, rows, v, dtype):
     assert torch.all(out.logprob < 0) and torch.all(out.logprob > -1e-7)
 
 
-@pytest.mark.parametrize("v", [5, 64, 1003, 9000, 70001])
+@pytest.mark.parametrize("v", [5, 64, 1003, 9000, 70001, 150001])
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 def test_masked_logits(dev, v, dtype):
     """-inf and the type's lowest number where a mask left nothing; rows with one
@@ -143,7 +143,7 @@ def test_masked_logits(dev, v, dtype):
     assert out.top_ids[4].tolist() == list(range(top)) and out.top_ids[5].tolist() == list(range(top))
 
 
-@pytest.mark.parametrize("v", [4, 300, 20011])
+@pytest.mark.parametrize("v", [4, 300, 20011, 150001])
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 def test_rows_without_a_distribution(dev, v, dtype):
     """NaN, +inf or nothing above -inf: NaN scores, as torch's log_softmax; NaN
@@ -442,7 +442,7 @@ def test_scores_of_a_model_are_its_loss(dev):
     s = g.score_tokens(model, idx, targets, top=3)
     loss = model(idx, targets)["loss"]
     n = (targets != -100).sum()
-    assert abs(float(-s.logprob.sum() / n - loss)) < 1e-5
+    assert abs((-s.logprob.sum() / n - loss).item()) < 1e-5
     nxt = g.score_tokens(model, idx)
     assert nxt.logprob.shape == (2, 19) and nxt.top_ids is None
     assert torch.equal(nxt.logprob[1], s.logprob[1, :-1])
@@ -511,13 +511,16 @@ def test_refusals(dev):
         with pytest.raises(error, match=text):
             bad()
     L = _lib.lib()
-    nb = L.tiq_token_logprobs_workspace(_lib.F32, 1, 50257, 5)
-    if nb:  # too little workspace: refused before any launch
-        y = torch.zeros(1, 50257, device=dev)
-        out = torch.full((8,), 3.0, device=dev)
-        ids = torch.zeros(8, dtype=torch.int64, device=dev)
-        rc = L.tiq_token_logprobs(y.data_ptr(), _lib.F32, 1, 1, 0, 50257, 50257, t.data_ptr(), -100, 5, out.data_ptr(),
-                                  out.data_ptr(), None, ids.data_ptr(), out.data_ptr(), None, 0, _lib.stream_of(y))
+    v = 131071  # a long row, cut into segments: too little workspace is refused before any launch
+    nb = L.tiq_token_logprobs_workspace(_lib.F32, 1, v, 5)
+    assert nb > 0 and L.tiq_token_logprobs_workspace(_lib.F32, 1, 50257, 5) == 0
+    y = torch.zeros(1, v, device=dev)
+    out = torch.full((8,), 3.0, device=dev)
+    ids = torch.zeros(8, dtype=torch.int64, device=dev)
+    for ws, n in ((None, nb), (out, nb - 1), (None, 0)):
+        rc = L.tiq_token_logprobs(y.data_ptr(), _lib.F32, 1, 1, 0, v, v, t.data_ptr(), -100, 5, out.data_ptr(),
+                                  out.data_ptr(), None, ids.data_ptr(), out.data_ptr(), _lib.ptr(ws), n,
+                                  _lib.stream_of(y))
         assert rc == _lib.EWORKSPACE and torch.all(out == 3.0)
 
 
@@ -539,12 +542,13 @@ def _check_top_on_gpu(x, out, top):
     assert ok
 
 
-@pytest.mark.parametrize("rows,threads", [(1030, 512), (600, 256), (40, 256), (3, 256)])
+@pytest.mark.parametrize("rows,v,threads", [(130, 20000, 512), (3, 20000, 512), (100, 200000, 256), (3, 200000, 256),
+                                            (130, 2400, 256), (20, 1000, 64)])
 @pytest.mark.parametrize("dtype", [FP32, BF16])
-def test_large_logits_in_few_places(dev, rows, threads, dtype):
+def test_large_logits_in_few_places(dev, rows, v, threads, dtype):
     """Rows whose large logits all fall to a few threads, ties by the thousand, rows with
     fewer tokens left than alternatives wanted: every way the selection can go."""
-    v, vec = 20000, 16 // (4 if dtype is FP32 else 2)
+    vec = 16 // (4 if dtype is FP32 else 2)
     gen = torch.Generator(device=dev).manual_seed(18)
     x = torch.randn(rows, v, generator=gen, device=dev)
     place = torch.arange(v, device=dev)
@@ -560,7 +564,7 @@ def test_large_logits_in_few_places(dev, rows, threads, dtype):
         _check_top_on_gpu(x, g.token_logprobs(x, torch.zeros(rows, dtype=torch.int64, device=dev), top=top), top)
 
 
-@pytest.mark.parametrize("rows,v", [(2, 40), (3, 1003), (2, 9001), (1030, 9001)])
+@pytest.mark.parametrize("rows,v", [(2, 40), (3, 1003), (2, 9001), (1030, 9001), (2, 150001)])
 def test_signalling_nans(dev, rows, v):
     """NaN bits of every kind give NaN scores and the top place, and touch no other row."""
     for dtype, bits in ((FP32, (0x7F800001, -0x3FFFFF, 0x7FC00000)), (BF16, (0x7F81, -0x7F, 0x7FC0))):
