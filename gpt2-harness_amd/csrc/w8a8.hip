@@ -81,15 +81,33 @@ __device__ __forceinline__ void load_16(const uint16_t* p, float (&v)[8]) {
     for (int i = 0; i < 8; ++i) v[i] = bf16_bits_to_f32(t.v[i]);
 }
 
+// What is applied to a row before it is quantized.
+enum Before { kAsIs, kLayerNorm, kGelu };
+struct LnArgs {
+    const float *w, *b;
+    float eps;
+};
+
+// Sum over each 16-lane row of the wavefront, in every lane of the row.
+__device__ __forceinline__ float row16_sum(float v) {
+    v += dpp_move<0xB1>(v);
+    v += dpp_move<0x4E>(v);
+    v += dpp_move<0x141>(v);
+    return v + dpp_move<0x140>(v);
+}
+
 // Four rows a workgroup, held in registers: 16 lanes of each wavefront on every row, so a
 // load instruction reads 256 consecutive bytes of each and a store covers 64-byte pieces
-// of the tiles. IT passes of TH / 4 lanes x 16 bytes a row; K >= 16 bytes of elements.
-template <bool TILES, int IT, int TH, typename TX>
+// of the tiles. IT passes of TH / 4 lanes x 16 bytes a row; K >= 16 bytes of elements. A
+// LayerNorm (mean and biased variance in two passes over the registers, as torch) or a
+// GELU before costs no pass over memory. 8192 x 6400 fp32 rows: 50 us, 5.2 TB/s.
+template <bool TILES, int IT, int TH, Before PRE, typename TX>
 __global__ __launch_bounds__(TH) void tokens_kernel(const TX* __restrict__ x, int64_t ldx, int M, int K,
                                                     int8_t* __restrict__ q, int64_t ldq, int64_t U,
-                                                    float* __restrict__ scale) {
+                                                    float* __restrict__ scale, LnArgs ln) {
     constexpr int VEC = 16 / (int)sizeof(TX), W = TH / 64, STEP = TH / 4 * VEC;
     __shared__ uint32_t red[W][4];
+    __shared__ float sums[PRE == kLayerNorm ? 2 : 1][W][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row = (int64_t)blockIdx.x * 4 + (lane >> 4);
     const int c0 = (wave * 16 + (lane & 15)) * VEC;
@@ -97,7 +115,6 @@ __global__ __launch_bounds__(TH) void tokens_kernel(const TX* __restrict__ x, in
     float v[IT][VEC];
 #pragma unroll
     for (int i = 0; i < IT; ++i) load_16(xr + min(c0 + STEP * i, K - VEC), v[i]);
-    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int c = c0 + STEP * i;
@@ -105,9 +122,50 @@ __global__ __launch_bounds__(TH) void tokens_kernel(const TX* __restrict__ x, in
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[i][e] = c + e < K ? load_x(xr + c + e) : 0.f;
         }
+    }
+    if constexpr (PRE == kLayerNorm) {
+        auto row_sum = [&](float t, int slot) {
+            t = row16_sum(t);
+            if ((lane & 15) == 0) sums[slot][wave][lane >> 4] = t;
+            __syncthreads();
+            t = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) t += sums[slot][w][lane >> 4];
+            return t;
+        };
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) t += v[i][e];
+        const float mu = row_sum(t, 0) / (float)K;
+        t = 0.f;
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) t = c0 + STEP * i + e < K ? fmaf(v[i][e] - mu, v[i][e] - mu, t) : t;
+        const float rstd = 1.0f / sqrtf(row_sum(t, 1) / (float)K + ln.eps);
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = c0 + STEP * i;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int k = min(c + e, K - 1);
+                v[i][e] = c + e < K ? fmaf((v[i][e] - mu) * rstd, ln.w[k], ln.b[k]) : 0.f;
+            }
+        }
+    }
+    if constexpr (PRE == kGelu) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[i][e] = gelu_tanh(v[i][e]);
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) m = umax(m, abs_bits(v[i][e]));
-    }
     m = row16_max_u32(m);
     if ((lane & 15) == 0) red[wave][lane >> 4] = m;
     __syncthreads();
@@ -172,6 +230,15 @@ __device__ __forceinline__ void store_y(uint16_t* p, float v) { *p = f32_to_bf16
 __device__ __forceinline__ float finish(int sum, float sx, float sw, float b) {
     return fmaf((float)sum * sx, sw, b);
 }
+
+// Added to an output last (fp32 outputs): element (m, n) at res + m ldr + n; null: nothing.
+struct Residual {
+    const float* res = nullptr;
+    int64_t ldr = 0;
+    __device__ __forceinline__ float operator()(float v, int64_t m, int n) const {
+        return res ? v + res[m * ldr + n] : v;
+    }
+};
 
 // Scales and codes in LDS of a product's rows (few of them: rows_fused): the W wavefronts
 // share a row where there are more of them than rows, else take rows in turn. Row m's
@@ -242,8 +309,8 @@ template <int W, bool FUSE, typename TX, typename TY>
 __global__ __launch_bounds__(64 * W) void w8a8_small(const TX* __restrict__ x, int64_t ldx,
                                                      const int8_t* __restrict__ xt, const float* __restrict__ sx,
                                                      const int8_t* __restrict__ wt, const float* __restrict__ sw,
-                                                     const float* __restrict__ bias, TY* __restrict__ y, int64_t ldy,
-                                                     int M, int N, int K, int U) {
+                                                     const float* __restrict__ bias, TY* y, int64_t ldy,
+                                                     int M, int N, int K, int U, Residual res) {
     constexpr int PF = 4;
     __shared__ int part[W][256];
     __shared__ float scale[FUSE ? kSmallRows : 1];
@@ -293,7 +360,7 @@ __global__ __launch_bounds__(64 * W) void w8a8_small(const TX* __restrict__ x, i
     int s = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) s += part[w][tid];
-    store_y(y + (int64_t)m * ldy + n, finish(s, FUSE ? scale[m] : sx[m], sw[n], bias ? bias[n] : 0.f));
+    store_y(y + (int64_t)m * ldy + n, res(finish(s, FUSE ? scale[m] : sx[m], sw[n], bias ? bias[n] : 0.f), m, n));
 }
 
 // The product without a staging step: W wavefronts share the K range of an output tile of
@@ -302,8 +369,8 @@ __global__ __launch_bounds__(64 * W) void w8a8_small(const TX* __restrict__ x, i
 template <int W, int TM, int TN, int PF, typename TY>
 __global__ __launch_bounds__(64 * W) void w8a8_direct(const int8_t* __restrict__ xt, const float* __restrict__ sx,
                                                       const int8_t* __restrict__ wt, const float* __restrict__ sw,
-                                                      const float* __restrict__ bias, TY* __restrict__ y, int64_t ldy,
-                                                      int M, int N, int U, int tiles_m) {
+                                                      const float* __restrict__ bias, TY* y, int64_t ldy,
+                                                      int M, int N, int U, int tiles_m, Residual res) {
     constexpr int G = TM * TN > 1 ? 2 : 1;  // sets of sums in LDS: one barrier a tile
     __shared__ int part[G][W][32 * 33];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -368,7 +435,8 @@ __global__ __launch_bounds__(64 * W) void w8a8_direct(const int8_t* __restrict__
                 int s = 0;
 #pragma unroll
                 for (int w = 0; w < W; ++w) s += set[w][(o >> 5) * 33 + (o & 31)];
-                if (m < M && n < N) store_y(y + (int64_t)m * ldy + n, finish(s, sx[m], sw[n], bias ? bias[n] : 0.f));
+                if (m < M && n < N)
+                    store_y(y + (int64_t)m * ldy + n, res(finish(s, sx[m], sw[n], bias ? bias[n] : 0.f), m, n));
             }
         }
 }
@@ -396,8 +464,8 @@ __device__ __forceinline__ void tile_of(int i, int tiles_m, int tiles_n, int& tm
 template <int TM, int TN, int D, int WD, int OCC, typename TY>
 __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict__ xt, const float* __restrict__ sx,
                                                         const int8_t* __restrict__ wt, const float* __restrict__ sw,
-                                                        const float* __restrict__ bias, TY* __restrict__ y, int64_t ldy,
-                                                        int M, int N, int U, int tiles_m, int tiles_n) {
+                                                        const float* __restrict__ bias, TY* y, int64_t ldy,
+                                                        int M, int N, int U, int tiles_m, int tiles_n, Residual res) {
     constexpr int STAGE = TM * 2048;             // bytes of a k64 step of rows
     constexpr int XL = STAGE / (256 * 16);       // staging loads a thread and step
     constexpr int NMF = TM * TN;                 // MFMAs a k32 block
@@ -548,10 +616,21 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
             for (int g = 0; g < 4; ++g) {
                 TY* dst = y + (int64_t)(m0 + 32 * i + 8 * g) * ldy + n0 + r;
                 if constexpr (sizeof(TY) == 4) {
+                    float add[4][TN];
+                    if (res.res) {
+                        const float* src = res.res + (int64_t)(m0 + 32 * i + 8 * g) * res.ldr + n0 + r;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int j = 0; j < TN; ++j) add[e][j] = src[(int64_t)e * res.ldr + 32 * j];
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int j = 0; j < TN; ++j) dst[(int64_t)e * ldy + 32 * j] = value(i, j, g, e);
+                        for (int j = 0; j < TN; ++j) {
+                            const float v = value(i, j, g, e);
+                            dst[(int64_t)e * ldy + 32 * j] = res.res ? v + add[e][j] : v;
+                        }
                 } else {
                     const bool odd = r & 1;  // even lanes store row e, odd ones row e + 1
                     dst += odd ? ldy - 1 : 0;
@@ -577,7 +656,8 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
                 const int m = m0 + 32 * i + 8 * g + e;
 #pragma unroll
                 for (int j = 0; j < TN; ++j)
-                    if (m < M && n0 + 32 * j + r < N) store_y(y + (int64_t)m * ldy + n0 + 32 * j + r, value(i, j, g, e));
+                    if (m < M && n0 + 32 * j + r < N)
+                        store_y(y + (int64_t)m * ldy + n0 + 32 * j + r, res(value(i, j, g, e), m, n0 + 32 * j + r));
             }
 }
 
@@ -589,29 +669,39 @@ size_t round256(size_t b) { return (b + 255) / 256 * 256; }
 // Rows a launch: its threads are counted in 32 bits.
 constexpr int64_t kTokenRows = 1 << 22;
 
+// Whether a row is held in registers while it is quantized: at most 32 passes of 256 threads
+// over its columns, with the padding of the tiles.
 template <bool TILES, typename TX>
-int launch_tokens(const TX* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
-                  hipStream_t st) {
+int64_t token_passes(int64_t K) {
     constexpr int VEC = 16 / (int)sizeof(TX);
-    const int64_t U = units_of(K);
-    // passes of 256 threads over the columns a row has, with its padding
-    const int64_t cols = TILES ? 32 * U : K, passes = (cols + 64 * VEC - 1) / (64 * VEC);
+    return ((TILES ? 32 * units_of(K) : K) + 64 * VEC - 1) / (64 * VEC);
+}
+template <bool TILES, typename TX>
+bool tokens_held(int64_t K) {
+    return K >= 16 / (int64_t)sizeof(TX) && token_passes<TILES, TX>(K) <= 32;
+}
+
+template <bool TILES, Before PRE, typename TX>
+int launch_tokens(const TX* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                  hipStream_t st, const LnArgs& ln = {}) {
+    const int64_t U = units_of(K), passes = token_passes<TILES, TX>(K);
+    if (PRE != kAsIs && !tokens_held<TILES, TX>(K)) return TIQ_EUNSUPPORTED;
     for (int64_t r0 = 0; r0 < rows; r0 += kTokenRows) {
         const int n = (int)std::min(rows - r0, kTokenRows);
         const TX* xr = x + r0 * ldx;
         int8_t* qr = q + (TILES ? r0 / 32 * U * 1024 : r0 * ldq);
         auto held = [&](auto kernel, int threads) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)((n + 3) / 4)), dim3(threads), 0, st, xr, ldx, n, (int)K, qr, ldq, U,
-                               scale + r0);
+                               scale + r0, ln);
         };
-        if (K < VEC || passes > 32)
+        if (!tokens_held<TILES, TX>(K))
             hipLaunchKernelGGL((tokens_generic<TILES, TX>), dim3((unsigned)n), dim3(256), 0, st, xr, ldx, K, qr, ldq, U,
                                scale + r0);
-        else if (passes <= 2) held(tokens_kernel<TILES, 2, 256, TX>, 256);
-        else if (passes <= 4) held(tokens_kernel<TILES, 4, 256, TX>, 256);
-        else if (passes <= 8) held(tokens_kernel<TILES, 8, 256, TX>, 256);
-        else if (passes <= 16) held(tokens_kernel<TILES, 4, 1024, TX>, 1024);
-        else held(tokens_kernel<TILES, 8, 1024, TX>, 1024);
+        else if (passes <= 2) held(tokens_kernel<TILES, 2, 256, PRE, TX>, 256);
+        else if (passes <= 4) held(tokens_kernel<TILES, 4, 256, PRE, TX>, 256);
+        else if (passes <= 8) held(tokens_kernel<TILES, 8, 256, PRE, TX>, 256);
+        else if (passes <= 16) held(tokens_kernel<TILES, 4, 1024, PRE, TX>, 1024);
+        else held(tokens_kernel<TILES, 8, 1024, PRE, TX>, 1024);
         const int rc = launch_status();
         if (rc != TIQ_OK) return rc;
     }
@@ -648,34 +738,46 @@ Path path_of(int64_t T, int64_t NT, int64_t K) {
     return (T + 1) / 2 * ((NT + 7) / 8) >= 150 ? kStaged64x256 : kStaged64x128;
 }
 
+// What stands around a product: before its rows are quantized, after its sums.
+struct Around {
+    Before pre = kAsIs;
+    LnArgs ln = {};
+    Residual res = {};
+};
+
 template <typename TX, typename TY>
 int run_w8a8(const TX* x, int64_t M, int64_t K, int64_t ldx, const int8_t* wt, const float* sw, const float* bias,
-             int64_t N, TY* y, int64_t ldy, uint8_t* ws, hipStream_t st) {
+             int64_t N, TY* y, int64_t ldy, uint8_t* ws, hipStream_t st, const Around& o = {}) {
     const int64_t U = units_of(K), T = tiles_of(M), NT = tiles_of(N);
     int8_t* xt = reinterpret_cast<int8_t*>(ws);
     float* sx = reinterpret_cast<float*>(ws + T * U * 1024);
     auto small = [&](auto kernel, int W, size_t lds) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((N + 15) / 16)), dim3(64 * W), lds, st, x, ldx, xt, sx, wt, sw, bias,
-                           y, ldy, (int)M, (int)N, (int)K, (int)U);
+                           y, ldy, (int)M, (int)N, (int)K, (int)U, o.res);
         return launch_status();
     };
-    if (rows_fused(sizeof(TX) == 4 ? TIQ_F32 : TIQ_BF16, M, K)) {
+    if (o.pre == kAsIs && rows_fused(sizeof(TX) == 4 ? TIQ_F32 : TIQ_BF16, M, K)) {
         const size_t lds = (size_t)(M * 32 * U);
         return K > 2048 ? small(w8a8_small<16, true, TX, TY>, 16, lds) : small(w8a8_small<8, true, TX, TY>, 8, lds);
     }
-    const int rc = launch_tokens<true>(x, M, K, ldx, xt, (int64_t)0, sx, st);
+    int rc = TIQ_EUNSUPPORTED;
+    if (o.pre == kAsIs) rc = launch_tokens<true, kAsIs>(x, M, K, ldx, xt, (int64_t)0, sx, st);
+    if constexpr (sizeof(TX) == 4 && sizeof(TY) == 4) {
+        if (o.pre == kLayerNorm) rc = launch_tokens<true, kLayerNorm>(x, M, K, ldx, xt, (int64_t)0, sx, st, o.ln);
+        if (o.pre == kGelu) rc = launch_tokens<true, kGelu>(x, M, K, ldx, xt, (int64_t)0, sx, st);
+    }
     if (rc != TIQ_OK) return rc;
     if (M <= kSmallRows) return K > 2048 ? small(w8a8_small<16, false, TX, TY>, 16, 0) : small(w8a8_small<8, false, TX, TY>, 8, 0);
     auto direct = [&](auto kernel, int TM, int TN) {
         const int64_t tm = (T + TM - 1) / TM, tn = (NT + TN - 1) / TN;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(512), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
-                           (int)N, (int)U, (int)tm);
+                           (int)N, (int)U, (int)tm, o.res);
         return launch_status();
     };
     auto staged = [&](auto kernel, int TM, int TN) {
         const int64_t tm = (T + TM - 1) / TM, tn = (NT + 4 * TN - 1) / (4 * TN);
         hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(256), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
-                           (int)N, (int)U, (int)tm, (int)tn);
+                           (int)N, (int)U, (int)tm, (int)tn, o.res);
         return launch_status();
     };
     switch (path_of(T, NT, K)) {
@@ -685,6 +787,15 @@ int run_w8a8(const TX* x, int64_t M, int64_t K, int64_t ldx, const int8_t* wt, c
         case kStaged64x256: return staged(w8a8_staged<2, 2, 4, 4, 2, TY>, 2, 2);
         default: return staged(w8a8_staged<4, 2, 3, 3, 2, TY>, 4, 2);
     }
+}
+
+size_t tiles_workspace(int64_t M, int64_t K) {
+    return round256((size_t)(tiles_of(M) * (units_of(K) * 1024 + 128)));  // (scales of whole tiles)
+}
+
+// (threads of a launch are counted in 32 bits)
+bool sizes_taken(int64_t M, int64_t K, int64_t N) {
+    return K <= kMaxK && M <= 0x7fffffc0LL && N <= 1 << 26 && tiles_of(M) * tiles_of(N) <= 1 << 26;
 }
 
 bool known_dtype(int d) { return d == TIQ_F32 || d == TIQ_BF16; }
@@ -702,8 +813,8 @@ extern "C" int tiq_quantize_tokens(const void* x, int x_dtype, int64_t rows, int
     if (!aligned(x, x_dtype == TIQ_F32 ? 4 : 2) || !aligned(scale, 4)) return TIQ_EALIGN;
     if (rows > 0x7fffffffLL) return TIQ_EUNSUPPORTED;
     if (x_dtype == TIQ_F32)
-        return launch_tokens<false>(static_cast<const float*>(x), rows, cols, ldx, q, ldq, scale, as_stream(stream));
-    return launch_tokens<false>(static_cast<const uint16_t*>(x), rows, cols, ldx, q, ldq, scale, as_stream(stream));
+        return launch_tokens<false, kAsIs>(static_cast<const float*>(x), rows, cols, ldx, q, ldq, scale, as_stream(stream));
+    return launch_tokens<false, kAsIs>(static_cast<const uint16_t*>(x), rows, cols, ldx, q, ldq, scale, as_stream(stream));
 }
 
 extern "C" size_t tiq_w8a8_tiles_bytes(int64_t N, int64_t K) {
@@ -732,7 +843,7 @@ extern "C" int tiq_w8a8_untile(const int8_t* tiles, int64_t N, int64_t K, int8_t
 
 extern "C" size_t tiq_linear_w8a8_workspace(int x_dtype, int64_t M, int64_t K, int64_t N) {
     if (!known_dtype(x_dtype) || M <= 0 || K <= 0 || N <= 0 || rows_fused(x_dtype, M, K)) return 0;
-    return round256((size_t)(tiles_of(M) * (units_of(K) * 1024 + 128)));  // (scales of whole tiles)
+    return tiles_workspace(M, K);
 }
 
 extern "C" int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const int8_t* w_tiles,
@@ -744,8 +855,7 @@ extern "C" int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K,
     if (!aligned(x, x_dtype == TIQ_F32 ? 4 : 2) || !aligned(y, y_dtype == TIQ_F32 ? 4 : 2) || !aligned(w_tiles, 16) ||
         !aligned(scale, 4) || !aligned(bias, 4))
         return TIQ_EALIGN;
-    // (threads of a launch are counted in 32 bits)
-    if (K > kMaxK || M > 0x7fffffc0LL || N > 1 << 26 || tiles_of(M) * tiles_of(N) > 1 << 26) return TIQ_EUNSUPPORTED;
+    if (!sizes_taken(M, K, N)) return TIQ_EUNSUPPORTED;
     const size_t need = tiq_linear_w8a8_workspace(x_dtype, M, K, N);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return TIQ_EWORKSPACE;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -758,4 +868,28 @@ extern "C" int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K,
     const uint16_t* xb = static_cast<const uint16_t*>(x);
     if (y_dtype == TIQ_F32) return run_w8a8(xb, M, K, ldx, w_tiles, scale, bias, N, static_cast<float*>(y), ldy, ws, st);
     return run_w8a8(xb, M, K, ldx, w_tiles, scale, bias, N, static_cast<uint16_t*>(y), ldy, ws, st);
+}
+
+extern "C" size_t tiq_linear_w8a8_prefill_workspace(int64_t M, int64_t K, int64_t N) {
+    if (M <= 0 || K <= 0 || N <= 0 || !tokens_held<true, float>(K) || !sizes_taken(M, K, N)) return 0;
+    return tiles_workspace(M, K);
+}
+
+extern "C" int tiq_linear_w8a8_prefill(const float* x, int64_t M, int64_t K, int64_t ldx, const int8_t* w_tiles,
+                                       const float* scale, const float* bias, int64_t N, float* y, int64_t ldy,
+                                       const float* ln_weight, const float* ln_bias, float ln_eps, int gelu,
+                                       const float* residual, int64_t ld_residual, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    if (M < 0 || K < 0 || N < 0 || (ln_weight == nullptr) != (ln_bias == nullptr) || (ln_weight && gelu))
+        return TIQ_EINVAL;
+    if (M == 0 || N == 0) return TIQ_OK;
+    if (K == 0 || !x || !w_tiles || !scale || !y || ldx < K || ldy < N || (residual && ld_residual < N)) return TIQ_EINVAL;
+    if (!aligned(x, 4) || !aligned(y, 4) || !aligned(w_tiles, 16) || !aligned(scale, 4) || !aligned(bias, 4) ||
+        !aligned(residual, 4) || !aligned(ln_weight, 4) || !aligned(ln_bias, 4))
+        return TIQ_EALIGN;
+    const size_t need = tiq_linear_w8a8_prefill_workspace(M, K, N);
+    if (!need) return TIQ_EUNSUPPORTED;
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) return TIQ_EWORKSPACE;
+    const Around o = {ln_weight ? kLayerNorm : gelu ? kGelu : kAsIs, {ln_weight, ln_bias, ln_eps}, {residual, ld_residual}};
+    return run_w8a8(x, M, K, ldx, w_tiles, scale, bias, N, y, ldy, static_cast<uint8_t*>(workspace), as_stream(stream), o);
 }

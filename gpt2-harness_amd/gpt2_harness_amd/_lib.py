@@ -89,6 +89,9 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "tiq_w8a8_untile": ([_vp, _i64, _i64, _vp, _vp], _i32),
     "tiq_linear_w8a8_workspace": ([_i32, _i64, _i64, _i64], _sz),
     "tiq_linear_w8a8": ([_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i32, _i64, _vp, _sz, _vp], _i32),
+    "tiq_linear_w8a8_prefill_workspace": ([_i64, _i64, _i64], _sz),
+    "tiq_linear_w8a8_prefill": ([_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _f32, _i32, _vp, _i64,
+                                 _vp, _sz, _vp], _i32),
     "tiq_token_logprobs_workspace": ([_i32, _i64, _i64, _i32], _sz),
     "tiq_token_logprobs": ([_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
                             _sz, _vp], _i32),

@@ -104,7 +104,9 @@ class QuantLinear(nn.Module):
         without the activation's own pass. None where that entry point does
         not apply; the caller then takes the two steps."""
         K, N = self.in_features, self.out_features
-        if (self.fmt == FMT_W8A8 or not x.is_cuda or x.dtype != torch.float32 or x.shape[-1] != K or K % 64
+        if self.fmt == FMT_W8A8:  # (forward_prefill applies it)
+            return None
+        if (not x.is_cuda or x.dtype != torch.float32 or x.shape[-1] != K or K % 64
                 or (torch.is_grad_enabled() and x.requires_grad)):
             return None
         lead = x.shape[:-1]
@@ -146,7 +148,9 @@ class QuantLinear(nn.Module):
         matrix cores as digit planes; the caller then takes the separate steps."""
         M, K = x2.shape
         N, fmt = self.out_features, self.fmt
-        if fmt == FMT_W8A8 or M <= 4 or K != self.in_features or (residual is not None and residual.shape[-1] != N):
+        if fmt == FMT_W8A8:
+            return None if kv is not None else _w8a8_prefill(self, x2, ln, gelu, residual)
+        if M <= 4 or K != self.in_features or (residual is not None and residual.shape[-1] != N):
             return None
         L = _lib.lib()
         ws_bytes = L.tiq_linear_workspace(_WF[fmt], _lib.F32, M, K, N)
@@ -248,6 +252,33 @@ def _w8a8_into(m: QuantLinear, x2: torch.Tensor, y: torch.Tensor) -> None:
                            None if ws is None else ws.data_ptr(), ws_bytes, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, f"quantized linear (w8a8, M={M}, K={K}, N={N})")
+
+
+def _w8a8_prefill(m: QuantLinear, x2: torch.Tensor, ln: nn.LayerNorm | None, gelu: bool,
+                  residual: torch.Tensor | None) -> torch.Tensor | None:
+    """:meth:`QuantLinear.forward_prefill` of a ``w8a8`` Linear
+    (``tiq_linear_w8a8_prefill``): LayerNorm or GELU as the rows are quantized, the
+    residual beside the scales."""
+    (M, K), N, dev = x2.shape, m.out_features, x2.get_device()
+    codes, scale, bias = m._buffers["codes"], m._buffers["scale"], m._parameters["bias"]
+    if (M <= 4 or K != m.in_features or codes.get_device() != dev or dev != torch._C._cuda_getDevice()
+            or (residual is not None and (residual.shape[-1] != N or residual.numel() != M * N
+                                          or not residual.is_contiguous()))):
+        return None
+    L = _lib.lib()
+    ws_bytes = L.tiq_linear_w8a8_prefill_workspace(M, K, N)
+    if not ws_bytes:
+        return None
+    y = x2.new_empty((M, N))
+    ws = x2.new_empty(ws_bytes, dtype=torch.uint8)
+    lw, lb, eps = (None, None, 0.0) if ln is None else (ln.weight.data_ptr(), ln.bias.data_ptr(), ln.eps)
+    rc = L.tiq_linear_w8a8_prefill(x2.data_ptr(), M, K, x2.stride(0), codes.data_ptr(), scale.data_ptr(),
+                                   None if bias is None else bias.data_ptr(), N, y.data_ptr(), N, lw, lb, eps, gelu,
+                                   None if residual is None else residual.data_ptr(), N, ws.data_ptr(), ws_bytes,
+                                   torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, f"quantized prefill linear (w8a8, M={M}, K={K}, N={N})")
+    return y
 
 
 def dequantize(m: QuantLinear) -> torch.Tensor:

@@ -636,6 +636,20 @@ int tiq_linear_w8a8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld
                     const float* scale, const float* bias, int64_t N, void* y, int y_dtype, int64_t ldy,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* tiq_linear_w8a8 over a prompt's fp32 rows with what stands around it in a block (as
+ * tiq_linear_prefill_ws for the weight-only formats): y = linear(pre(x)) + residual, pre
+ * the LayerNorm of the rows (ln_weight and ln_bias (K); NULL: none) or gelu_tanh (gelu
+ * != 0; bit for bit tiq_gelu_tanh first), applied as the rows are quantized, and
+ * residual (M, N) added last (NULL: none; it may be y itself). Not both a LayerNorm and a
+ * GELU. The workspace query returns 0 for sizes it does not take (K < 4 or > 8192), for
+ * which the call returns TIQ_EUNSUPPORTED. */
+size_t tiq_linear_w8a8_prefill_workspace(int64_t M, int64_t K, int64_t N);
+int tiq_linear_w8a8_prefill(const float* x, int64_t M, int64_t K, int64_t ldx, const int8_t* w_tiles,
+                            const float* scale, const float* bias, int64_t N, float* y, int64_t ldy,
+                            const float* ln_weight, const float* ln_bias, float ln_eps, int gelu,
+                            const float* residual, int64_t ld_residual, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 /* -------------------------------------------------------- token scores */
 
 /* Log probabilities of given tokens under rows of logits, the entropy of each row

@@ -68,6 +68,30 @@ def test_linear_w8a8_arguments():
     assert call(M=1 << 31, N=1 << 20, ldy=1 << 20, nb=1 << 60) == EUNSUPPORTED
 
 
+def test_linear_w8a8_prefill_arguments():
+    L = _lib.load()
+    f = L.tiq_linear_w8a8_prefill
+    need = L.tiq_linear_w8a8_prefill_workspace(3, 64, 5)
+    assert need >= 32 * 64 + 32 * 4
+    for size in ((0, 64, 5), (3, 3, 5), (3, 8193, 5), (3, 64, 0)):
+        assert L.tiq_linear_w8a8_prefill_workspace(*size) == 0
+    ok = dict(x=16, M=3, K=64, ldx=64, w=16, s=16, b=None, N=5, y=16, ldy=5, lw=None, lb=None, eps=1e-5, gelu=0, r=None,
+              ldr=0, ws=16, nb=need)
+
+    def call(**kw):
+        return f(*{**ok, **kw}.values(), None)
+
+    assert call(M=0) == 0 and call(N=0) == 0
+    for bad in (dict(M=-1), dict(K=0), dict(x=None), dict(w=None), dict(s=None), dict(y=None), dict(ldx=63), dict(ldy=4),
+                dict(lw=16), dict(lb=16), dict(lw=16, lb=16, gelu=1), dict(r=16, ldr=4)):
+        assert call(**bad) == EINVAL, bad
+    for bad in (dict(x=18), dict(w=24), dict(y=18), dict(r=18, ldr=5), dict(lw=18, lb=16)):
+        assert call(**bad) == EALIGN, bad
+    for bad in (dict(ws=None), dict(nb=need - 1), dict(ws=24)):
+        assert call(**bad) == EWORKSPACE, bad
+    assert call(K=8256, ldx=8256, nb=1 << 40) == EUNSUPPORTED and call(K=3) == EUNSUPPORTED
+
+
 def test_token_scores_arguments():
     L = _lib.load()
     ok = dict(x=16, d=0, batch=1, rows=2, sb=0, sr=9, v=9, t=16, ignore=-100, top=0, lp=16, h=16, st=None, ids=None,

@@ -17,6 +17,7 @@ import torch
 
 import gpt2_harness_amd as g
 from gpt2_harness_amd import _lib
+from gpt2_harness_amd.model import gelu_tanh
 from oracle import model as OM
 from oracle import quant as OQ
 
@@ -244,6 +245,105 @@ def test_captured_calls_and_other_streams(dev, m):
     assert torch.equal(y, want[3])
 
 
+# ------------------------------------------------- a prompt's rows, fused
+FUSED = [(5, 64, 33), (16, 768, 96), (17, 100, 65), (77, 1001, 130), (130, 1600, 257), (400, 768, 768), (1030, 320, 1100),
+         (1500, 1600, 2400), (600, 6400, 320), (2100, 256, 1100)]
+
+
+@pytest.mark.parametrize("m,k,n", FUSED)
+def test_gelu_and_residual_are_the_separate_steps(dev, m, k, n):
+    """Bit for bit: GELU as the rows are quantized, the residual beside the scales."""
+    x = _rows(m, k, 30).to(dev)
+    q, s, b = _weight(n, k, 31)
+    lin = _linear(q, s, b, dev)
+    gen = torch.Generator().manual_seed(32)
+    res = torch.randn(m, n, generator=gen).to(dev)
+    act = gelu_tanh(x)
+    assert torch.equal(lin.forward_prefill(x, gelu=True), lin(act))
+    assert torch.equal(lin.forward_prefill(x, residual=res), lin(x) + res)
+    assert torch.equal(lin.forward_prefill(x, gelu=True, residual=res), lin(act) + res)
+    assert torch.equal(lin.forward_prefill(x), lin(x))
+    # the residual's place as the output's
+    L = _lib.lib()
+    nb = L.tiq_linear_w8a8_prefill_workspace(m, k, n)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    y = res.clone()
+    rc = L.tiq_linear_w8a8_prefill(x.data_ptr(), m, k, k, lin.codes.data_ptr(), lin.scale.data_ptr(),
+                                   lin.bias.data_ptr(), n, y.data_ptr(), n, None, None, 0.0, 0, y.data_ptr(), n,
+                                   ws.data_ptr(), nb, _lib.stream_of(x))
+    assert rc == 0 and torch.equal(y, lin(x) + res)
+
+
+@pytest.mark.parametrize("m,k,n", FUSED)
+@pytest.mark.parametrize("shift", [0.0, 3.0])
+def test_layer_norm_before_the_product(dev, m, k, n, shift):
+    """Against a LayerNorm in 64 bits and the codes' product. The fp32 LayerNorm is off by
+    at most e = (|h| + |b|) 8 u + |w| (k + 40) u (|mean| + |x|) rstd, u = 2^-24: its sums of k
+    terms, the subtraction, rsqrt and the affine step; so is a row's largest value, and
+    the scale with it. A code is another than the exact one only where its quotient lies
+    within that distance, over the scale, of a half, plus the quotient's own 3 u: each
+    such code may move its outputs by sx sw |qw|, and the scale moves all by its part."""
+    gen = torch.Generator().manual_seed(33)
+    x = _rows(m, k, 34) + shift
+    q, s, b = _weight(n, k, 35)
+    lin = _linear(q, s, b, dev)
+    ln = torch.nn.LayerNorm(k).to(dev)
+    w, c = 1 + 0.1 * torch.randn(k, generator=gen), 0.1 * torch.randn(k, generator=gen)
+    with torch.no_grad():
+        ln.weight.copy_(w)
+        ln.bias.copy_(c)
+    with torch.no_grad():
+        y = lin.forward_prefill(x.to(dev), ln=ln).double()
+    u = 2.0**-24
+    xd, wd, cd = x.to(dev).double(), w.to(dev).double(), c.to(dev).double()
+    mu = xd.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(xd.var(1, unbiased=False, keepdim=True) + ln.eps)
+    h = (xd - mu) * rstd * wd + cd
+    e = (h.abs() + cd.abs()) * 8 * u + wd.abs() * (k + 40) * u * (mu.abs() + xd.abs()) * rstd
+    top = h.abs().amax(1, keepdim=True)
+    rel = e.amax(1, keepdim=True) / top + 2 * u  # of the scale
+    sx = top / 127
+    t = h / sx
+    qx = torch.round(t)
+    near = (((t - torch.floor(t)) - 0.5).abs() <= e / sx + t.abs() * (rel + 3 * u)).double()
+    qw, sw = q.to(dev).double(), s.to(dev).double()
+    core = (qx @ qw.t()) * sx * sw
+    want = core + b.to(dev).double()
+    bound = (near @ qw.abs().t()) * sx * sw + core.abs() * (rel + 2 * u) + want.abs() * 2 * u
+    bad = ((y - want).abs() > bound * (1 + 1e-6) + 1e-30).sum().item()
+    assert bad == 0, f"{bad} outputs beyond the bound"
+    assert near.mean() < 0.05  # few codes are in doubt
+
+
+def test_fused_rows_that_are_not_ordinary(dev):
+    q, s, b = _weight(70, 96, 36)
+    lin = _linear(q, s, b, dev)
+    x = _rows(40, 96, 37)
+    x[1, 5], x[2, 90], x[3], x[4] = float("inf"), float("nan"), 0.0, 5.0
+    x = x.to(dev)
+    ln = torch.nn.LayerNorm(96).to(dev).requires_grad_(False)
+    y = lin.forward_prefill(x, ln=ln)
+    assert torch.isnan(y[1:3]).all() and torch.isfinite(y[3:]).all()
+    y = lin.forward_prefill(x, gelu=True)
+    assert torch.isnan(y[1:3]).all() and torch.isfinite(y[5:]).all()
+    assert torch.equal(y[3], b.to(dev))
+
+
+def test_prompts_that_the_fused_call_leaves_alone(dev):
+    """Four rows and fewer, long rows, a cache's slots: None, and the module's own steps."""
+    q, s, b = _weight(8, 8256, 38)
+    lin = _linear(q, s, b, dev)
+    x = _rows(6, 8256, 39).to(dev)
+    assert lin.forward_prefill(x, gelu=True) is None and lin.forward_gelu_in(x) is None
+    assert not lin.writes_kv(600)
+    q, s, b = _weight(64, 64, 40)
+    lin = _linear(q, s, b, dev)
+    assert lin.forward_prefill(_rows(4, 64, 41).to(dev), gelu=True) is None
+    x = _rows(300, 64, 42).to(dev)
+    assert lin.forward_prefill(x, kv=(x, x, 300)) is None
+    assert lin.forward_prefill(x, residual=x[:1]) is None
+
+
 # ---------------------------------------------------------------- model paths
 def _tiny(dev, seed=0):
     torch.manual_seed(seed)
@@ -297,6 +397,25 @@ def test_generation_through_the_captured_decoder(dev, batch):
     assert torch.equal(dec.run(prompt, 12), out)
     eager = g.generate(qm, prompt, 12)
     assert (eager == out).float().mean() > 0.9  # equal but for codes on a border
+
+
+@pytest.mark.parametrize("batch,length", [(1, 7), (2, 40), (5, 64)])
+def test_fused_prompt_blocks_are_the_separate_modules(dev, batch, length):
+    """A prompt through the blocks with everything inside the Linears, against the same
+    model with a hook on every module, which runs them one by one."""
+    qm, _ = g.quantize_model(_tiny(dev, 6), 8, act_bits=8)
+    idx = (torch.arange(batch * length, device=dev) * 13 % 211).view(batch, length)
+    with torch.no_grad():
+        cache, plain_cache = g.KVCache.empty(2), g.KVCache.empty(2)
+        fused = qm(idx, cache=cache)["logits"]
+        hooks = [m.register_forward_hook(lambda *a: None) for m in qm.modules()]
+        plain = qm(idx, cache=plain_cache)["logits"]
+        for h in hooks:
+            h.remove()
+    assert not torch.equal(fused, torch.zeros_like(fused))
+    assert (fused - plain).abs().max() < 2e-3  # equal but for codes on a border (1/127 of a row's largest)
+    for a, b in zip(cache.keys + cache.values, plain_cache.keys + plain_cache.values):
+        assert (a - b).abs().max() < 2e-2
 
 
 def test_cached_steps_equal_the_whole_window(dev):
