@@ -304,7 +304,8 @@ __device__ __forceinline__ void quantize_rows(const TX* __restrict__ x, int64_t 
 // range dealt out to them in k64 blocks, their sums added through LDS. The weights are
 // read once, by the wavefront that multiplies them, PF blocks on their way at a time.
 // FUSE (few rows): the workgroup quantizes the rows itself, behind the first weights'
-// loads, which spares a launch; else their tiles come from tokens_kernel.
+// loads, which spares a launch; else their tiles come from tokens_kernel. A launch's own
+// cost and two trips to memory bound it (768 x 2304, one row: 3.6 us in a graph).
 template <int W, bool FUSE, typename TX, typename TY>
 __global__ __launch_bounds__(64 * W) void w8a8_small(const TX* __restrict__ x, int64_t ldx,
                                                      const int8_t* __restrict__ xt, const float* __restrict__ sx,
@@ -365,7 +366,8 @@ __global__ __launch_bounds__(64 * W) void w8a8_small(const TX* __restrict__ x, i
 
 // The product without a staging step: W wavefronts share the K range of an output tile of
 // TM x TN 32 x 32 tiles, each with its own operand loads, PF units on their way at a
-// time, and add their sums through LDS, a 32 x 32 tile after the other.
+// time, and add their sums through LDS, a 32 x 32 tile after the other. No barrier until
+// the sums: what bounds it is a trip to L2 a turn, then L2's rate (128 x 6400 x 1600: 11 us).
 template <int W, int TM, int TN, int PF, typename TY>
 __global__ __launch_bounds__(64 * W) void w8a8_direct(const int8_t* __restrict__ xt, const float* __restrict__ sx,
                                                       const int8_t* __restrict__ wt, const float* __restrict__ sw,
@@ -459,8 +461,16 @@ __device__ __forceinline__ void tile_of(int i, int tiles_m, int tiles_n, int& tm
 // 32 TM rows x 128 TN columns, a wavefront all the rows and 32 TN columns. The rows' tiles
 // pass through LDS (double buffered, one barrier a k64 step; loaded D - 1 steps before
 // their LDS store), as all four wavefronts need them; the weights' go straight from
-// memory into the registers of the one wavefront that needs them, WD - 1/2 steps ahead: 1 KB of consecutive memory an instruction either way, no bank conflicts, no
-// swizzle. Beside each MFMA goes one of the step's other operations.
+// memory into the registers of the one wavefront that needs them, WD - 1/2 steps ahead:
+// 1 KB of consecutive memory an instruction either way, no bank conflicts, no swizzle.
+// Beside each MFMA goes one of the step's other operations. Two workgroups a CU, so that
+// one's epilogue runs beside the other's MFMAs.
+// What bounds it: 8192 x 6400 x 1600 in 128 x 256 tiles takes 81 us (2.07 POP/s; the
+// platform's int8 product 88), and 74 of them with every load left out: the MFMAs at the
+// clock that the chip holds under them (64 us of 81 on rows and codes of zeros), and the
+// two rounds that 1.6 tiles a SIMD make. 4096 x 1600 x 4800 to bf16: 38 us, 34 without
+// loads; its epilogue took 25 us more when every scale was a load of its own and a store
+// two bytes a lane.
 template <int TM, int TN, int D, int WD, int OCC, typename TY>
 __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict__ xt, const float* __restrict__ sx,
                                                         const int8_t* __restrict__ wt, const float* __restrict__ sw,

@@ -4,7 +4,7 @@
 probability of the row's token, the entropy of the row and its most probable
 alternatives; where autograd follows the logits, one more pass gives their
 gradient. The reference computes the first of these inside ``F.cross_entropy``
-(``src/transformer_internals/model.py:591-597``, ``quantization.py:262-319``),
+(``src/transformer_internals/model.py:593-598``, ``quantization.py:262-319``),
 which writes the whole ``log_softmax`` to memory on the way; entropy and
 alternatives are an extension. :func:`score_tokens` applies it to a model and
 token windows. :func:`~gpt2_harness_amd.sampling.generate` (``scores=``) and

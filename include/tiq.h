@@ -654,7 +654,7 @@ int tiq_linear_w8a8_prefill(const float* x, int64_t M, int64_t K, int64_t ldx, c
 
 /* Log probabilities of given tokens under rows of logits, the entropy of each row
  * and its `top` most probable alternatives (log_softmax and gather inside the
- * reference's F.cross_entropy, model.py:591-597; entropy and alternatives are an
+ * reference's F.cross_entropy, model.py:593-598; entropy and alternatives are an
  * extension). Row (b, r), b < batch, r < rows, starts at logits + b stride_batch +
  * r stride_row (elements; the vocabulary's stride is 1) and takes place b rows + r
  * of every other array; fp32 or bf16 logits at any alignment of their elements.
