@@ -134,7 +134,9 @@ class QuantLinear(nn.Module):
 
     def writes_kv(self, M: int) -> bool:
         """Whether :meth:`forward_prefill` over ``M`` rows takes ``kv``."""
-        return self.fmt != FMT_W8A8 and bool(_lib.lib().tiq_linear_prefill_writes_kv(_WF[self.fmt], M, self.in_features, self.out_features))
+        if self.fmt == FMT_W8A8:
+            return False
+        return bool(_lib.lib().tiq_linear_prefill_writes_kv(_WF[self.fmt], M, self.in_features, self.out_features))
 
     def forward_prefill(self, x2: torch.Tensor, ln: nn.LayerNorm | None = None, gelu: bool = False,
                         residual: torch.Tensor | None = None,
@@ -232,6 +234,10 @@ def tile_codes(codes: torch.Tensor) -> torch.Tensor:
     return tiles
 
 
+def _scales_are_fp32(scale: torch.Tensor, bias: torch.Tensor | None) -> bool:
+    return scale.dtype is torch.float32 and (bias is None or bias.dtype is torch.float32)
+
+
 def _w8a8_into(m: QuantLinear, x2: torch.Tensor, y: torch.Tensor) -> None:
     """The ``w8a8`` product: ``x2``'s rows quantized, then multiplied as integers."""
     codes, scale, bias = m._buffers["codes"], m._buffers["scale"], m._parameters["bias"]
@@ -241,6 +247,8 @@ def _w8a8_into(m: QuantLinear, x2: torch.Tensor, y: torch.Tensor) -> None:
     if dev != torch._C._cuda_getDevice():  # launches go to the current device
         with torch.cuda.device(dev):
             return _w8a8_into(m, x2, y)
+    if not _scales_are_fp32(scale, bias):  # (a module cast to another type)
+        raise TypeError(f"a w8a8 Linear keeps its scale and bias in float32, got {scale.dtype}")
     L = _lib.lib()
     M, K = x2.shape
     N, xd = m.out_features, _lib.dtype_code(x2.dtype)
@@ -262,7 +270,7 @@ def _w8a8_prefill(m: QuantLinear, x2: torch.Tensor, ln: nn.LayerNorm | None, gel
     (M, K), N, dev = x2.shape, m.out_features, x2.get_device()
     codes, scale, bias = m._buffers["codes"], m._buffers["scale"], m._parameters["bias"]
     if (M <= 4 or K != m.in_features or codes.get_device() != dev or dev != torch._C._cuda_getDevice()
-            or (residual is not None and (residual.shape[-1] != N or residual.numel() != M * N
+            or not _scales_are_fp32(scale, bias) or (residual is not None and (residual.shape[-1] != N or residual.numel() != M * N
                                           or not residual.is_contiguous()))):
         return None
     L = _lib.lib()
@@ -287,6 +295,8 @@ def dequantize(m: QuantLinear) -> torch.Tensor:
     out = torch.empty((N, K), dtype=torch.float32, device=m.codes.device)
     st = _lib.stream_of(out)
     if m.fmt == FMT_W8A8:
+        if m.scale.dtype is not torch.float32:
+            raise TypeError(f"a w8a8 Linear keeps its scale in float32, got {m.scale.dtype}")
         codes = torch.empty((N, K), dtype=torch.int8, device=m.codes.device)
         _lib.check(L.tiq_w8a8_untile(m.codes.data_ptr(), N, K, codes.data_ptr(), st), "w8a8 codes")
         rc = L.tiq_dequantize_int8(codes.data_ptr(), m.scale.data_ptr(), 1, N, K, out.data_ptr(), st)

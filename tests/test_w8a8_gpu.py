@@ -475,6 +475,23 @@ def test_refusals(dev):
         _linear(q, s, b, dev)(torch.zeros(2, 16))
 
 
+@pytest.mark.parametrize("m", [2, 40])
+def test_a_module_cast_to_another_type_is_refused(dev, m):
+    """The kernels read the scales and the bias as float32: a cast module would send
+    them past the buffers' ends."""
+    for bias in (torch.zeros(24, device=dev), None):
+        lin = g.QuantLinear(torch.ones(24, 64, dtype=torch.int8, device=dev), torch.ones(24, device=dev), bias, 64, 24, 8,
+                            "per_channel", "w8a8").to(torch.bfloat16)
+        x = torch.ones(m, 64, device=dev)
+        with pytest.raises(TypeError, match="float32"):
+            lin(x)
+        with pytest.raises(TypeError, match="float32"):
+            lin(x.bfloat16())
+        with pytest.raises(TypeError, match="float32"):
+            lin.weight
+        assert lin.forward_prefill(x) is None
+
+
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 def test_more_rows_than_one_launch_takes(dev, dtype):
     m, k, n = (1 << 22) + 37, 12, 3
