@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -148,7 +149,10 @@ def token_logprobs(
         ``logits`` (first order; ``top_ids`` is a choice and carries none).
 
     ``-inf`` logits are probabilities of 0. A row that holds NaN or ``+inf``, or
-    nothing above ``-inf``, has NaN scores.
+    nothing above ``-inf``, has NaN scores. A training step captured into a graph takes
+    its gradients with ``torch.autograd.grad``, or lets no eager step's results of the
+    same leaves live meanwhile: autograd would accumulate into them on the eager
+    step's stream, which a capture does not survive.
     """
     if not (isinstance(logits, torch.Tensor) and isinstance(tokens, torch.Tensor) and logits.is_cuda
             and tokens.is_cuda):
@@ -170,6 +174,8 @@ def token_logprobs(
         raise ValueError("logits hold no vocabulary")
     if not 0 <= top <= min(V, MAX_TOP):
         raise ValueError(f"top must be in [0, {min(V, MAX_TOP)}], got {top}")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(logits).tangent is not None:
+        raise RuntimeError("token_logprobs has no forward-mode derivative")
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     if logits.requires_grad and torch.is_grad_enabled():

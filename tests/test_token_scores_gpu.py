@@ -542,6 +542,17 @@ def _check_top_on_gpu(x, out, top):
     assert ok
 
 
+def test_tangents_are_refused(dev):
+    from torch.autograd import forward_ad
+    x, tokens = _logits(2, 20, 18)
+    x, tokens = x.to(dev), tokens.to(dev)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            g.token_logprobs(dual, tokens)
+        assert torch.isfinite(g.token_logprobs(x, tokens).logprob).all()
+
+
 @pytest.mark.parametrize("rows,v,threads", [(130, 20000, 512), (3, 20000, 512), (100, 200000, 256), (3, 200000, 256),
                                             (130, 2400, 256), (20, 1000, 64)])
 @pytest.mark.parametrize("dtype", [FP32, BF16])
