@@ -803,9 +803,9 @@ size_t tiles_workspace(int64_t M, int64_t K) {
     return round256((size_t)(tiles_of(M) * (units_of(K) * 1024 + 128)));  // (scales of whole tiles)
 }
 
-// (threads of a launch are counted in 32 bits)
+// (threads of a launch are counted in 32 bits: 64 an output column, for few rows)
 bool sizes_taken(int64_t M, int64_t K, int64_t N) {
-    return K <= kMaxK && M <= 0x7fffffc0LL && N <= 1 << 26 && tiles_of(M) * tiles_of(N) <= 1 << 26;
+    return K <= kMaxK && M <= 0x7fffffc0LL && N <= 1 << 25 && tiles_of(M) * tiles_of(N) <= 1 << 26;
 }
 
 bool known_dtype(int d) { return d == TIQ_F32 || d == TIQ_BF16; }

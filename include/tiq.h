@@ -624,7 +624,7 @@ int tiq_w8a8_untile(const int8_t* tiles, int64_t N, int64_t K, int8_t* q, void* 
 /* A Linear on int8 activations and int8 weights, the activations quantized in the
  * call: y = (sum_k qx qw) sx sw + bias with (qx, sx) of each row of x as
  * tiq_quantize_tokens gives them, w_tiles (tiq_w8a8_tile) and scale (N) the weight's
- * codes and channel scales. The integer sums are exact (K <= 131072); an output
+ * codes and channel scales. The integer sums are exact (K <= 131072, N <= 2^25); an output
  * takes three roundings in fp32 (the sum, times sx, times sw plus the bias) and one
  * more where y is bf16. No counterpart in the reference: it takes the place of
  * F.linear on W_hat (model.py:254,319,352,355) where activations may be coded too.
@@ -678,7 +678,8 @@ int tiq_token_logprobs(const void* logits, int dtype, int64_t batch, int64_t row
  * vocab), contiguous, in the logits' type:
  *   [j = t] g + sum_i [j = a_i] g_i - p_j (g + sum_i g_i + h (log p_j + entropy))
  * with g = g_logprob (0 for an ignored token, NaN for one outside the vocabulary),
- * h = g_entropy, g_i = g_top of alternative a_i; each of the three may be NULL.
+ * h = g_entropy, g_i = g_top of alternative a_i (the forward's: no two alike); each of
+ * the three may be NULL. grad is not the logits' memory.
  * The probabilities are computed again from the logits and the forward's stats. */
 int tiq_token_logprobs_grad(const void* logits, int dtype, int64_t batch, int64_t rows, int64_t stride_batch,
                             int64_t stride_row, int64_t vocab, const int64_t* tokens, int64_t ignore_index,

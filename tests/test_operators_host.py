@@ -66,6 +66,7 @@ def test_linear_w8a8_arguments():
         assert call(**bad) == EWORKSPACE, bad
     assert call(K=131073, ldx=131073, nb=1 << 40) == EUNSUPPORTED
     assert call(M=1 << 31, N=1 << 20, ldy=1 << 20, nb=1 << 60) == EUNSUPPORTED
+    assert call(M=4, N=(1 << 25) + 1, ldy=1 << 26) == EUNSUPPORTED
 
 
 def test_linear_w8a8_prefill_arguments():
