@@ -471,19 +471,16 @@ __device__ __forceinline__ void tile_of(int i, int tiles_m, int tiles_n, int& tm
 // two rounds that 1.6 tiles a SIMD make. 4096 x 1600 x 4800 to bf16: 38 us, 34 without
 // loads; its epilogue took 25 us more when every scale was a load of its own and a store
 // two bytes a lane.
-template <int TM, int TN, int D, int WD, int OCC, typename TY>
-__global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict__ xt, const float* __restrict__ sx,
-                                                        const int8_t* __restrict__ wt, const float* __restrict__ sw,
-                                                        const float* __restrict__ bias, TY* y, int64_t ldy,
-                                                        int M, int N, int U, int tiles_m, int tiles_n, Residual res) {
+template <int TM, int TN, int D, int WD, typename TY>
+__device__ __forceinline__ void staged_product(int8_t* smem, int t0, int tn, const int8_t* __restrict__ xt,
+                                               const float* __restrict__ sx, const int8_t* __restrict__ wt,
+                                               const float* __restrict__ sw, const float* __restrict__ bias, TY* y,
+                                               int64_t ldy, int M, int N, int U, const Residual& res) {
     constexpr int STAGE = TM * 2048;             // bytes of a k64 step of rows
     constexpr int XL = STAGE / (256 * 16);       // staging loads a thread and step
     constexpr int NMF = TM * TN;                 // MFMAs a k32 block
     static_assert(STAGE % 4096 == 0, "whole loads a thread");
-    __shared__ __attribute__((aligned(1024))) int8_t smem[2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int tm, tn;
-    tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int T = (M + 31) / 32, NT = (N + 31) / 32, nk = U / 2;
 
     // rows' tile i of the workgroup: 2 KB a step; thread: 16 bytes of tile q (XL of them)
@@ -491,7 +488,7 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
 #pragma unroll
     for (int q = 0; q < XL; ++q) {
         const int o = q * 4096 + tid * 16;
-        xp[q] = xt + (int64_t)min(tm * TM + o / 2048, T - 1) * U * 1024 + o % 2048;  // past the last: it again (not stored)
+        xp[q] = xt + (int64_t)min(t0 + o / 2048, T - 1) * U * 1024 + o % 2048;  // past the last: it again (not stored)
     }
     const int8_t* wp[TN];
 #pragma unroll
@@ -600,7 +597,7 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
     // are asked for all at once, whole tiles are stored without a test, and bf16
     // neighbours of two rows swap a value each, so that a store takes four bytes a lane.
     const int r = lane & 31, h = lane >> 5;
-    const int m0 = tm * TM * 32 + 4 * h, n0 = (tn * 4 + wave) * TN * 32;
+    const int m0 = t0 * 32 + 4 * h, n0 = (tn * 4 + wave) * TN * 32;
     float scw[TN], b[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -613,12 +610,12 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            s4[i][g] = *reinterpret_cast<const float4*>(sx + min(tm * TM + i, T - 1) * 32 + 8 * g + 4 * h);
+            s4[i][g] = *reinterpret_cast<const float4*>(sx + min(t0 + i, T - 1) * 32 + 8 * g + 4 * h);
     auto value = [&](int i, int j, int g, int e) {
         const float sxe = e == 0 ? s4[i][g].x : e == 1 ? s4[i][g].y : e == 2 ? s4[i][g].z : s4[i][g].w;
         return finish(acc[i][j][4 * g + e], sxe, scw[j], b[j]);
     };
-    const bool whole = (tm + 1) * TM * 32 <= M && n0 + 32 * TN <= N;
+    const bool whole = (t0 + TM) * 32 <= M && n0 + 32 * TN <= N;
     if (whole && (sizeof(TY) == 4 || (((uintptr_t)y | (uint64_t)ldy * 2) & 3) == 0)) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -669,6 +666,30 @@ __global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict
                     if (m < M && n0 + 32 * j + r < N)
                         store_y(y + (int64_t)m * ldy + n0 + 32 * j + r, res(value(i, j, g, e), m, n0 + 32 * j + r));
             }
+}
+
+// A workgroup a tile (tile_of); TAIL: of each XCD's tiles the first `whole`, then the others
+// in halves of TM / 2 (whole_of).
+template <int TM, int TN, int D, int WD, int OCC, bool TAIL, typename TY>
+__global__ __launch_bounds__(256, OCC) void w8a8_staged(const int8_t* __restrict__ xt, const float* __restrict__ sx,
+                                                        const int8_t* __restrict__ wt, const float* __restrict__ sw,
+                                                        const float* __restrict__ bias, TY* y, int64_t ldy, int M, int N,
+                                                        int U, int tiles_m, int tiles_n, int whole, Residual res) {
+    __shared__ __attribute__((aligned(1024))) int8_t smem[2 * TM * 2048];
+    int tm, tn, i = blockIdx.x;
+    if constexpr (TAIL) {
+        if (i >= 8 * whole) {
+            const int local = (i >> 3) - whole, half = local & 1;
+            i = (whole + (local >> 1)) * 8 + (i & 7);
+            if (i >= tiles_m * tiles_n) return;
+            tile_of(i, tiles_m, tiles_n, tm, tn);
+            if ((tm * TM + half * (TM / 2)) * 32 >= M) return;
+            staged_product<TM / 2, TN, 4, 4>(smem, tm * TM + half * (TM / 2), tn, xt, sx, wt, sw, bias, y, ldy, M, N, U, res);
+            return;
+        }
+    }
+    tile_of(i, tiles_m, tiles_n, tm, tn);
+    staged_product<TM, TN, D, WD>(smem, tm * TM, tn, xt, sx, wt, sw, bias, y, ldy, M, N, U, res);
 }
 
 // Workgroups of 256 for n pieces of work; each goes on to further ones past 2^20 of them.
@@ -724,8 +745,9 @@ int launch_tokens(const TX* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, 
 //     600, 384 x 1600 x 1600: 10.6 against 11.2 .. 12.2 staged; 1600, 1024 x 1600 x 1600:
 //     17.1 against 12.4); 2 x 2 tiles a workgroup where K is long (512 x 6400 x 1600: 22.9
 //     against 28.1);
-//   128 x 256 staged tiles where those are many and K is not short (1024 x 1600 x 4800:
-//     20.2 against 24.9 with 64 x 256; 8192 x 768 x 2304: 37.5 against 33.5);
+//   128 x 256 staged tiles where those are many (152 of them, 1024 x 1600 x 4800: 21.6
+//     against 22.9 with 64 x 256; 256, 2048 x 1024 x 4096: 22.4 against 22.0, to bf16 18.7
+//     against 20.3; 128, 1001 x 1024 x 4096: 19.5 against 14.7);
 //   64 x 256 where those are many (2048 x 1600 x 1600, 224 of them: 17.4 against 18.7 with
 //     64 x 128; 1024 x 1600 x 1600, 112: 13.6 against 12.4), else 64 x 128.
 // Whether the product quantizes its rows itself (then it takes no workspace): up to 8
@@ -744,8 +766,18 @@ Path path_of(int64_t T, int64_t NT, int64_t K) {
     if (T * NT <= 400) return kDirect;
     if (K >= 3200 && T * NT <= 1200) return kDirectLong;
     if (T * NT <= 800) return kDirect;
-    if (K >= 1280 && (T + 3) / 4 * ((NT + 7) / 8) >= 150) return kStaged128x256;
+    if ((T + 3) / 4 * ((NT + 7) / 8) >= 150) return kStaged128x256;
     return (T + 1) / 2 * ((NT + 7) / 8) >= 150 ? kStaged64x256 : kStaged64x128;
+}
+
+// 128 x 256 tiles: how many of an XCD's, which its 32 CUs take in rounds, are taken whole,
+// the rest in halves, or -1: all of them whole. A last round of halves, one a CU at most,
+// takes half the time (4096 x 1600 x 4800 fp32, 12 of 76 tiles an XCD: 47.6 us against 50.6;
+// 4096 x 6400 x 2304, 4 of 36: 86.5 against 97.3); two a CU do not (8192 x 1600 x 1600, 24 of
+// 56: 45.1 against 40.6).
+int64_t whole_of(int64_t T, int64_t NT) {
+    const int64_t tiles = ((T + 3) / 4 * ((NT + 7) / 8) + 7) / 8, whole = tiles / 32 * 32;
+    return whole && tiles > whole && tiles - whole <= 16 ? whole : -1;
 }
 
 // What stands around a product: before its rows are quantized, after its sums.
@@ -786,16 +818,20 @@ int run_w8a8(const TX* x, int64_t M, int64_t K, int64_t ldx, const int8_t* wt, c
     };
     auto staged = [&](auto kernel, int TM, int TN) {
         const int64_t tm = (T + TM - 1) / TM, tn = (NT + 4 * TN - 1) / (4 * TN);
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(256), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
-                           (int)N, (int)U, (int)tm, (int)tn, o.res);
+        const int64_t whole = TM == 4 ? whole_of(T, NT) : -1;
+        const int64_t groups = whole < 0 ? tm * tn : 8 * (2 * ((tm * tn + 7) / 8) - whole);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, st, xt, sx, wt, sw, bias, y, ldy, (int)M,
+                           (int)N, (int)U, (int)tm, (int)tn, (int)whole, o.res);
         return launch_status();
     };
     switch (path_of(T, NT, K)) {
         case kDirect: return direct(w8a8_direct<8, 1, 1, 4, TY>, 1, 1);
         case kDirectLong: return direct(w8a8_direct<8, 2, 2, 2, TY>, 2, 2);
-        case kStaged64x128: return staged(w8a8_staged<2, 1, 4, 4, 2, TY>, 2, 1);
-        case kStaged64x256: return staged(w8a8_staged<2, 2, 4, 4, 2, TY>, 2, 2);
-        default: return staged(w8a8_staged<4, 2, 3, 3, 2, TY>, 4, 2);
+        case kStaged64x128: return staged(w8a8_staged<2, 1, 4, 4, 2, false, TY>, 2, 1);
+        case kStaged64x256: return staged(w8a8_staged<2, 2, 4, 4, 2, false, TY>, 2, 2);
+        default:
+            if (whole_of(T, NT) >= 0) return staged(w8a8_staged<4, 2, 3, 3, 2, true, TY>, 4, 2);
+            return staged(w8a8_staged<4, 2, 3, 3, 2, false, TY>, 4, 2);
     }
 }
 

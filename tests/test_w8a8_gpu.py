@@ -130,7 +130,10 @@ def test_product_against_64_bits(dev, m, k, n, dtype):
     _check(y, x, q, s, b)
 
 
-@pytest.mark.parametrize("m,k,n", [(2100, 256, 1100), (4096, 192, 768), (1500, 1600, 2400), (700, 6400, 1600)])
+@pytest.mark.parametrize("m,k,n", [(2100, 256, 1100), (4096, 192, 768), (1500, 1600, 2400), (700, 6400, 1600),
+                                   # 128 x 256 tiles: all whole; the last ones in halves, with ragged edges, in
+                                   # uneven shares of the XCDs
+                                   (4096, 96, 4096), (4096, 192, 4800), (4001, 130, 4701), (2500, 70, 3700)])
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 def test_large_product_against_64_bits(dev, m, k, n, dtype):
     """The products of many rows, checked on the GPU in 64 bits."""
@@ -247,7 +250,7 @@ def test_captured_calls_and_other_streams(dev, m):
 
 # ------------------------------------------------- a prompt's rows, fused
 FUSED = [(5, 64, 33), (16, 768, 96), (17, 100, 65), (77, 1001, 130), (130, 1600, 257), (400, 768, 768), (1030, 320, 1100),
-         (1500, 1600, 2400), (600, 6400, 320), (2100, 256, 1100)]
+         (1500, 1600, 2400), (600, 6400, 320), (2100, 256, 1100), (2500, 68, 3700)]
 
 
 @pytest.mark.parametrize("m,k,n", FUSED)
