@@ -597,7 +597,11 @@ __device__ __forceinline__ void staged_product(int8_t* smem, int t0, int tn, con
 
     // result register q of lane (r, h): row 8 (q / 4) + 4 h + q % 4, column r. The scales
     // are asked for all at once, whole tiles are stored without a test, and bf16
-    // neighbours of two rows swap a value each, so that a store takes four bytes a lane.
+    // neighbours of two rows swap a value each, so that a store takes four bytes a lane. Past
+    // the caches, as every workgroup of a round stores at once and the next one's operands are
+    // read meanwhile (8192 x 6400 x 1600 fp32 126 us against 135, to bf16 115.5 against 117;
+    // 1001 x 1024 x 4096 fp32 13.5 against 14.6; eight GPT-2-XL blocks over 4096 rows 2.64 ms
+    // against 2.69).
     const int r = lane & 31, h = lane >> 5;
     const int m0 = t0 * 32 + 4 * h, n0 = (tn * 4 + wave) * TN * 32;
     float scw[TN], b[TN];
@@ -638,7 +642,7 @@ __device__ __forceinline__ void staged_product(int8_t* smem, int t0, int tn, con
 #pragma unroll
                         for (int j = 0; j < TN; ++j) {
                             const float v = value(i, j, g, e);
-                            dst[(int64_t)e * ldy + 32 * j] = res.res ? v + add[e][j] : v;
+                            __builtin_nontemporal_store(res.res ? v + add[e][j] : v, dst + (int64_t)e * ldy + 32 * j);
                         }
                 } else {
                     const bool odd = r & 1;  // even lanes store row e, odd ones row e + 1
@@ -649,8 +653,8 @@ __device__ __forceinline__ void staged_product(int8_t* smem, int t0, int tn, con
                         for (int j = 0; j < TN; ++j) {
                             const float v0 = value(i, j, g, e), v1 = value(i, j, g, e + 1);
                             const float got = dpp_move<0xB1>(odd ? v0 : v1);
-                            *reinterpret_cast<uint32_t*>(dst + (int64_t)e * ldy + 32 * j) =
-                                odd ? pk_bf16(got, v1) : pk_bf16(v0, got);
+                            __builtin_nontemporal_store(odd ? pk_bf16(got, v1) : pk_bf16(v0, got),
+                                                        reinterpret_cast<uint32_t*>(dst + (int64_t)e * ldy + 32 * j));
                         }
                 }
             }
