@@ -465,12 +465,12 @@ __device__ __forceinline__ void tile_of(int i, int tiles_m, int tiles_n, int& tm
 // 1 KB of consecutive memory an instruction either way, no bank conflicts, no swizzle.
 // Beside each MFMA goes one of the step's other operations. Two workgroups a CU, so that
 // one's epilogue runs beside the other's MFMAs.
-// What bounds it: 8192 x 6400 x 1600 in 128 x 256 tiles takes 81 us (2.07 POP/s; the
+// What bounds it: 8192 x 6400 x 1600 in 128 x 256 tiles takes 79 us (2.12 POP/s; the
 // platform's int8 product 88), and 74 of them with every load left out: the MFMAs at the
-// clock that the chip holds under them (64 us of 81 on rows and codes of zeros), and the
+// clock that the chip holds under them (on rows and codes of zeros 17 us less), and the
 // two rounds that 1.75 tiles a CU make; over the launch the MFMAs are busy 0.48 of the cycles,
-// at 2.0 GHz. 4096 x 1600 x 4800 to bf16: 36 us (38 before its last round was halved), 34
-// without loads; its epilogue took 25 us more when every scale was a load of its own and a
+// at 2.0 GHz. 4096 x 1600 x 4800 to bf16 takes 35 us: 13 its launch and its outputs, the k-loop
+// 20 without MFMAs, about as much without loads, 25 with both. Its epilogue took 25 us more when every scale was a load of its own and a
 // store two bytes a lane. K split over two or four groups of wavefronts of a workgroup
 // gained at 1024 x 6400 x 1600 only (27.4 us against 32.5) and lost 1 to 10 us elsewhere.
 template <int TM, int TN, int D, int WD, typename TY>

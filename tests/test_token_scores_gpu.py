@@ -416,6 +416,33 @@ def test_gradient_replayed_from_a_graph(dev):
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows,v", [(3, 150001), (40, 20011)])
+def test_scores_replayed_from_graphs(dev, rows, v):
+    """Two captured calls (rows in segments with a workspace; whole rows) replayed in
+    turn with new logits, eager calls between, on another stream than the capture's."""
+    graphs = []
+    for seed in (19, 20):
+        x, tokens = _logits(rows, v, seed)
+        x, tokens = x.to(dev), tokens.to(dev)
+        g.token_logprobs(x, tokens, top=5)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = g.token_logprobs(x, tokens, top=5)
+        graphs.append((graph, x, tokens, out))
+    side = torch.cuda.Stream()
+    for turn in range(3):
+        for i, (graph, x, tokens, out) in enumerate(graphs):
+            x.copy_(_logits(rows, v, 200 + 2 * turn + i)[0])
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+            want = g.token_logprobs(x, tokens, top=5)  # beside the replay
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+
+
 def test_changed_logits_are_refused_in_the_backward(dev):
     x, tokens = _logits(3, 50, 16)
     base = x.to(dev).requires_grad_()
