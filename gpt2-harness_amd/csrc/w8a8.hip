@@ -445,7 +445,8 @@ __global__ __launch_bounds__(64 * W) void w8a8_direct(const int8_t* __restrict__
 
 // Tile index -> tile: eight contiguous ranges, one an XCD (workgroups go round the XCDs),
 // each walked in groups of four row tiles, so that the workgroups of an XCD that run
-// together share rows and weights in its L2.
+// together share rows and weights in its L2 (groups of 8, 12 or 16, nearer to a square, are
+// level or 1 to 5% slower: 4096 x 1600 x 4800 to bf16 45.1 / 46.6 / 47.3 / 47.3 us).
 __device__ __forceinline__ void tile_of(int i, int tiles_m, int tiles_n, int& tm, int& tn) {
     constexpr int XCDS = 8, G = 4;
     const int total = tiles_m * tiles_n, q = total / XCDS, r = total % XCDS;
